@@ -18,7 +18,10 @@ STAMP = LIB + '.srchash'
 SOURCES = ['gemm_f32.hip', 'gemm_pipe.hip', 'gemm_small.hip', 'gemm_ks.hip', 'gemm_n192.hip', 'gemv_f32.hip', 'attention.hip', 'vocab.hip', 'decode.hip', 'decode_persistent.hip',
            'targets.hip', 'prof.hip', 'backward.hip', 'gru.hip', 'rowwise.hip', 'flash_attn_pad.hip', 'compact.hip', 'enc_attn_bwd.hip', 'ingest.hip', 'beam.hip', 'train_fused.hip', 'optim.hip', 'stream_mm.hip', 'gemm_dxs.hip', 'train_rows.hip', 'lstm_seq.hip']
 HEADERS = ['gvd_common.h', 'gemm_common.h', 'gemv_f32.h', 'top2.h', 'decode_persistent.h', 'philox.h', 'enc_dropout.h']
-CFLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result']
+# -packed-fp32-ops: no packed fp32 instructions (v_pk_add / mul / fma_f32), which the compiler otherwise forms by itself from
+# ordinary float code and some of whose forms have given wrong results on this hardware now and then
+CFLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result',
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # decode_persistent.hip keeps ~150 weight registers per lane for the whole launch; the SLP vectorizer would pair its
 # accumulators into v_pk_fma_f32 and splat every resident weight into a register PAIR (2x the footprint -> spills)
 EXTRA = {'decode_persistent.hip': ['-fno-slp-vectorize']}
