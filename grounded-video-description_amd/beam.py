@@ -35,7 +35,7 @@ def _state(stack):
 
 
 def _fork(st, parent):
-    return _state(st['stack'].index_select(1, parent))
+    return _state(ops.reorder_rows([st['stack']], parent, dim=1)[0])
 
 
 def _core_rows(P, st, xt, fc_gates, pre, pmask_rows, K, att2_out):

@@ -108,6 +108,46 @@ class OptGroup(C.Structure):
                 ('count', C.c_int), ('part0', C.c_int)]
 
 
+GRAD_MAX_TENSORS, GRAD_CHUNK = 120, 8192
+
+
+class GradGroup(C.Structure):
+    """gvd_grad_group: up to 120 gradient tensors of one launch of the norm / the clipping, passed by value."""
+    _fields_ = [('src', C.c_void_p * GRAD_MAX_TENSORS), ('dst', C.c_void_p * GRAD_MAX_TENSORS),
+                ('n', C.c_int64 * GRAD_MAX_TENSORS), ('chunk0', C.c_uint32 * (GRAD_MAX_TENSORS + 1)),
+                ('src_type', C.c_uint8 * GRAD_MAX_TENSORS), ('dst_type', C.c_uint8 * GRAD_MAX_TENSORS), ('count', C.c_int)]
+
+
+class GradClip(C.Structure):
+    _fields_ = [('max_norm', C.c_double), ('inv_scale', C.c_double)]
+
+
+EMBEDDING_MAX, EMBEDDING_MAX_WIDTH = 1 << 25, 1 << 20
+BEAM_SELECT_MAX = 32
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [('logits', C.c_void_p), ('ld', C.c_int64), ('dtype', C.c_int), ('B', C.c_int), ('K', C.c_int), ('V', C.c_int),
+                ('W', C.c_int), ('eos', C.c_int), ('scores', c_f32p), ('finished', c_u8p), ('out_scores', c_f32p),
+                ('parent', c_i64p), ('word', c_i64p), ('out_finished', c_u8p), ('workspace', C.c_void_p),
+                ('workspace_bytes', C.c_size_t)]
+
+
+REORDER_MAX_TENSORS = 16
+
+
+class ReorderTensor(C.Structure):
+    _fields_ = [('src', C.c_void_p), ('dst', C.c_void_p), ('outer', C.c_int64), ('src_outer', C.c_int64),
+                ('dst_outer', C.c_int64), ('src_row', C.c_int64), ('dst_row', C.c_int64), ('row_bytes', C.c_int64),
+                ('unit', C.c_int)]
+
+
+class ReorderGroup(C.Structure):
+    """gvd_reorder_group: up to 16 state tensors of one launch, passed by value."""
+    _fields_ = [('t', ReorderTensor * REORDER_MAX_TENSORS), ('tile0', C.c_int64 * (REORDER_MAX_TENSORS + 1)),
+                ('count', C.c_int)]
+
+
 # every symbol include/gvd_hip.h declares: (restype, argtypes)
 _SIG = {
     'gvd_version': (C.c_char_p, []),
@@ -230,10 +270,23 @@ _SIG = {
     'gvd_clip_coef': (C.c_int, [c_f32p, C.c_int, C.c_float, c_f32p, C.c_void_p]),
     'gvd_adam_step': (C.c_int, [C.c_void_p, c_f32p, C.c_void_p, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float,
                                 C.c_void_p]),
+    'gvd_embedding_fwd': (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_float,
+                                    C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
+    'gvd_embedding_bwd_workspace_bytes': (C.c_size_t, [C.c_int64, C.c_int64, C.c_int]),
+    'gvd_embedding_bwd': (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                                    C.c_int, C.c_int, C.c_float, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t,
+                                    C.c_void_p]),
+    'gvd_grad_chunk': (C.c_int, []),
+    'gvd_grad_parts': (C.c_int, [C.POINTER(GradGroup)]),
+    'gvd_grad_sumsq': (C.c_int, [C.POINTER(GradGroup), C.c_void_p, C.c_void_p]),
+    'gvd_grad_scale': (C.c_int, [C.POINTER(GradGroup), C.POINTER(GradClip), C.c_void_p, C.c_int, c_f32p, C.c_void_p]),
+    'gvd_beam_select_workspace_bytes': (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    'gvd_beam_select': (C.c_int, [C.POINTER(BeamSelectArgs), C.c_void_p]),
+    'gvd_reorder_rows': (C.c_int, [C.POINTER(ReorderGroup), c_i64p, C.c_int64, C.c_int64, C.c_void_p]),
 }
 
 EXPORTS = tuple(_SIG)
-ABI_VERSION = 20        # must equal gvd_abi_version() of the loaded library (struct layouts above are part of the ABI)
+ABI_VERSION = 21        # must equal gvd_abi_version() of the loaded library (struct layouts above are part of the ABI)
 _lib = None
 
 
@@ -283,6 +336,15 @@ def check(rc, what):
 
 def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+# element types of the kernels that take 32- and 16-bit tensors (GVD_F32 / GVD_BF16 / GVD_F16)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def stream_on(device):
+    """The current stream of `device` (which need not be the current device)."""
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def ptr(t):

@@ -7,8 +7,8 @@ import os
 
 import torch
 
-from .hip import (AttnSide, DxGroup, GemmArgs, GemmSeg, GreedyArgs, GvdHipError, LstmArgs, check, lib, ptr, require_cuda_f32,
-                  stream_ptr)
+from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs, DxGroup, GemmArgs, GemmSeg, GreedyArgs,
+                  GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr, require_cuda_f32, stream_on, stream_ptr)
 
 # ---------------------------------------------------------------------------------------------------------------------
 # "No library GEMM on the hot path" as an invariant.  Every place where a product or softmax of the path would leave
@@ -1848,3 +1848,261 @@ def check_masked_rows_zero(x, pnt_mask, flag):
     assert x.is_contiguous()
     check(lib().gvd_check_masked_rows_zero(ptr(x), D, C.c_void_p(pnt_mask.data_ptr() + 1), pnt_mask.shape[1], B, R,
                                            ptr(flag), stream_ptr()), 'gvd_check_masked_rows_zero')
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Token-side operators of training and search, for fp32 / bf16 / fp16 tensors (csrc/embedding.hip, csrc/beam_select.hip).
+# They run on the current stream of their tensors' device, whichever device is current; scratch memory is allocated per call, so
+# calls on several streams and captured graphs share none.
+# ---------------------------------------------------------------------------------------------------------------------
+def _check_embedding(tokens, weight, act, padding_idx):
+    """The lookup's arguments; returns padding_idx as a row of the table (None -> -1)."""
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise GvdHipError('embedding: tokens must be int64 or int32, got %s' % tokens.dtype)
+    if weight.dtype not in DTYPES or weight.dim() != 2:
+        raise GvdHipError('embedding: the table must be a 2-D float32 / bfloat16 / float16 tensor, got %s of %d dimensions'
+                          % (weight.dtype, weight.dim()))
+    if act not in (0, 1):
+        raise GvdHipError('embedding: act must be 0 (none) or 1 (ReLU), got %r' % (act,))
+    pad, V = -1, weight.shape[0]
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise GvdHipError('embedding: padding_idx %d is outside a table of %d rows' % (padding_idx, V))
+        pad = padding_idx % V
+    if tokens.numel() > EMBEDDING_MAX or V > EMBEDDING_MAX or weight.shape[1] > EMBEDDING_MAX_WIDTH:
+        raise GvdHipError('embedding: at most %d tokens and rows of %d columns, got %d tokens and a table %s'
+                          % (EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, tokens.numel(), tuple(weight.shape)))
+    if not V and tokens.numel():
+        raise GvdHipError('embedding: the table has no rows')
+    if not (tokens.is_cuda and weight.is_cuda):
+        raise GvdHipError('embedding: non-GPU tensor; there is no CPU fallback')
+    if tokens.device != weight.device:
+        raise GvdHipError('embedding: tokens on %s, table on %s' % (tokens.device, weight.device))
+    return pad
+
+
+def _embedding_fwd(tokens, weight, scale, act):
+    """The launch.  tokens any shape (contiguous), weight [V, E] with contiguous rows."""
+    V, E = weight.shape
+    n = tokens.numel()
+    out = torch.empty(tokens.shape + (E,), dtype=weight.dtype, device=weight.device)
+    if n and E:
+        with torch.cuda.device(weight.device):
+            check(lib().gvd_embedding_fwd(ptr(tokens), tokens.dtype == torch.int64, n, ptr(weight), weight.stride(0) if V > 1 else E, V,
+                                          E, DTYPES[weight.dtype], scale, act, ptr(out), E, stream_on(weight.device)),
+                  'gvd_embedding_fwd')
+    return out
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, act, pad):
+        ctx.save_for_backward(tokens, weight if act else None)
+        ctx.meta = (weight.shape, weight.dtype, scale, act, pad)
+        return _embedding_fwd(tokens, weight, scale, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        tokens, weight = ctx.saved_tensors
+        (V, E), dtype, scale, act, pad = ctx.meta
+        n, dev = tokens.numel(), dy.device
+        if not n or not E or not V:
+            return None, torch.zeros(V, E, dtype=dtype, device=dev), None, None, None
+        dy2 = dy.reshape(n, E)
+        if E > 1 and dy2.stride(1) != 1:       # (a gradient broadcast over the rows, stride 0, is read in place)
+            dy2 = dy2.contiguous()
+        dw = torch.empty(V, E, dtype=dtype, device=dev)
+        need = lib().gvd_embedding_bwd_workspace_bytes(n, V, E)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            check(lib().gvd_embedding_bwd(ptr(tokens), tokens.dtype == torch.int64, n, ptr(dy2), dy2.stride(0), ptr(weight),
+                                          (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype], scale, act, pad, ptr(dw), ptr(ws),
+                                          ws.numel(), stream_on(dev)), 'gvd_embedding_bwd')
+        return None, dw, None, None, None
+
+
+def embedding(tokens, weight, scale=1.0, act=0, padding_idx=None):
+    """act(scale * weight[tokens]) - the word embedding with its scaling and ReLU (model.py:79-82: Embedding + ReLU) in one
+    launch, differentiable with respect to `weight`.
+
+    tokens int64 / int32 of any shape, weight [V, E] fp32 / bf16 / fp16 (a column block of a wider table is read in place);
+    act 1 = ReLU; padding_idx: a row that gets no gradient.  The result has weight's type, [..., E], rounded once.
+    Gradient: positions sorted by token, every row of the table summed in fp32 in a fixed order - the same bits at every
+    run - and written once.  A token outside [0, V) is not an error the host can see without waiting: its row of the result
+    is NaN and it adds nothing to the gradient.  At most 2^25 tokens and rows."""
+    pad = _check_embedding(tokens, weight, act, padding_idx)
+    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
+    V, E = weight.shape
+    if E > 1 and weight.stride(1) != 1 or V > 1 and weight.stride(0) < E:
+        weight = weight.contiguous()
+    scale = float(scale)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(tokens, weight, scale, act, pad)
+    return _embedding_fwd(tokens, weight, scale, act)
+
+
+def beam_select(logits, scores, width=None, finished=None, eos=None):
+    """The selection of one beam-search step over beams and vocabulary: for each of B samples the `width` best of the K * V
+    candidates scores[b,q] + log_softmax(logits)[b,q,v], descending, equal ones by q * V + v ascending.
+
+    logits [B*K, V] or [B, K, V], fp32 / bf16 / fp16, contiguous rows (any row stride); scores f32 [B, K] (the beams' summed
+    log-probabilities; -inf: not in use yet); width: K unless given.  finished (u8 / bool [B, K]): an ended beam goes on with
+    the word `eos` at its score and nothing else; its logits are not read.  A beam whose score or log-sum-exp is not finite
+    (NaN or +inf logits, all words banned) has -inf for every word.  Candidates are scored and compared in fp64.
+
+    Returns (scores f32 [B, W], parent i64 [B, W], word i64 [B, W], finished [B, W]): parent = the row b*K + q the candidate
+    extends, as reorder_rows takes it; finished = of the type given (u8 if none was), None without eos.
+    K, W <= 32; B * K <= 65535."""
+    if logits.dtype not in DTYPES or scores.dtype != torch.float32 or scores.dim() != 2:
+        raise GvdHipError('beam_select: logits must be float32 / bfloat16 / float16 and scores float32 [B, K], got %s and %s %s'
+                          % (logits.dtype, scores.dtype, tuple(scores.shape)))
+    B, K = scores.shape
+    V = logits.shape[-1]
+    W = K if width is None else int(width)
+    if logits.shape != (B * K, V) and logits.shape != (B, K, V):
+        raise GvdHipError('beam_select: logits %s do not fit scores %s' % (tuple(logits.shape), tuple(scores.shape)))
+    if not (B > 0 and 0 < K <= BEAM_SELECT_MAX and 0 < W <= BEAM_SELECT_MAX and W <= K * V and B * K <= 65535):
+        raise GvdHipError('beam_select: %d samples of %d beams, width %d, %d words: needs 1 <= beams, width <= %d, width <= beams * '
+                          'words, samples * beams <= 65535' % (B, K, W, V, BEAM_SELECT_MAX))
+    if finished is not None and (finished.shape != (B, K) or finished.dtype not in (torch.uint8, torch.bool)):
+        raise GvdHipError('beam_select: finished must be uint8 / bool [B, K], got %s %s' % (finished.dtype, tuple(finished.shape)))
+    if eos is None and finished is not None or eos is not None and not 0 <= eos < V:
+        raise GvdHipError('beam_select: eos must be a word of the vocabulary (and given where finished is), got %r' % (eos,))
+    if not (logits.is_cuda and scores.is_cuda and (finished is None or finished.is_cuda)):
+        raise GvdHipError('beam_select: non-GPU tensor; there is no CPU fallback')
+    dev = logits.device
+    if scores.device != dev or (finished is not None and finished.device != dev):
+        raise GvdHipError('beam_select: tensors on different devices')
+    if logits.dim() == 3:
+        logits = logits.reshape(B * K, V)
+    if V > 1 and logits.stride(1) != 1 or B * K > 1 and logits.stride(0) < V:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    a = BeamSelectArgs()
+    a.logits, a.ld, a.dtype = ptr(logits), max(logits.stride(0), V), DTYPES[logits.dtype]
+    a.B, a.K, a.V, a.W, a.eos = B, K, V, W, -1 if eos is None else eos
+    a.scores = ptr(scores)
+    if finished is not None:
+        finished = finished.contiguous()
+        a.finished = ptr(finished)
+    out = torch.empty(B, W, dtype=torch.float32, device=dev)
+    ids = torch.empty(2, B, W, dtype=torch.int64, device=dev)
+    parent, word = ids.unbind(0)
+    done = None
+    if eos is not None:
+        done = torch.empty(B, W, dtype=torch.uint8 if finished is None else finished.dtype, device=dev)
+        a.out_finished = ptr(done)
+    need = lib().gvd_beam_select_workspace_bytes(B, K, V, W)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    a.out_scores, a.parent, a.word = ptr(out), ptr(parent), ptr(word)
+    a.workspace, a.workspace_bytes = ptr(ws), need
+    with torch.cuda.device(dev):
+        check(lib().gvd_beam_select(C.byref(a), stream_on(dev)), 'gvd_beam_select')
+    return out, parent, word, done
+
+
+def _rows_view(x, dim):
+    """(outer, outer stride, row stride, row bytes) in bytes of x seen as [outer, rows = x.shape[dim], row]; None where its
+    strides do not allow that view."""
+    size = x.element_size()
+    inner = 1
+    for d in range(x.dim() - 1, dim, -1):
+        if x.shape[d] != 1 and x.stride(d) != inner:
+            return None
+        inner *= x.shape[d]
+    outer, ostride = 1, 0
+    for d in range(dim - 1, -1, -1):
+        if x.shape[d] == 1:
+            continue
+        if outer == 1:
+            ostride = x.stride(d)
+        elif x.stride(d) != ostride * outer:
+            return None
+        outer *= x.shape[d]
+    return outer, ostride * size, x.stride(dim) * size, inner * size
+
+
+def _extent(x):
+    """[first, last) byte address of a tensor's elements."""
+    first = x.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
+def reorder_rows(states, parent, dim=0, out=None):
+    """[x.index_select(dim, parent) for x in states] in one launch: the beams' states, caches and histories follow their
+    parents (CaptionModelBU.py:75-96).
+
+    states: tensors of any type whose dimension `dim` holds the same number of rows; parent int64, any shape (its entries in
+    order are the new rows: beam_select's parent goes in as it is).  out: tensors of the result's shape and type, which must not
+    overlap the states (two sets of buffers, swapped from step to step); otherwise new ones.  Returns the list of results.
+    A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1)."""
+    states = list(states)
+    dev = parent.device
+    if parent.dtype != torch.int64:
+        raise GvdHipError('reorder_rows: parent must be int64, got %s' % parent.dtype)
+    if not states:
+        return []
+    parent = parent.reshape(-1)
+    if not parent.is_contiguous():
+        parent = parent.contiguous()
+    n = parent.numel()
+    if out is not None and len(out) != len(states):
+        raise GvdHipError('reorder_rows: %d states, %d results' % (len(states), len(out)))
+    rows = None
+    results, items = [], []
+    for i, x in enumerate(states):
+        if x.device != dev:
+            raise GvdHipError('reorder_rows: parent on %s, state %d on %s' % (dev, i, x.device))
+        if not -x.dim() <= dim < x.dim():
+            raise GvdHipError('reorder_rows: state %d has %d dimensions, no dimension %d' % (i, x.dim(), dim))
+        d = dim % x.dim()
+        if rows is None:
+            rows = x.shape[d]
+        if x.shape[d] != rows:
+            raise GvdHipError('reorder_rows: state %d has %d rows, the first one %d' % (i, x.shape[d], rows))
+        shape = x.shape[:d] + (n,) + x.shape[d + 1:]
+        if out is None:
+            y = torch.empty(shape, dtype=x.dtype, device=dev)
+        else:
+            y = out[i]
+            if y.shape != shape or y.dtype != x.dtype or y.device != dev:
+                raise GvdHipError('reorder_rows: result %d must be %s %s on %s' % (i, x.dtype, tuple(shape), dev))
+        results.append(y)
+        if y.numel() == 0:
+            continue
+        if rows == 0:
+            raise GvdHipError('reorder_rows: the states have no rows')
+        src = _rows_view(x, d)
+        if src is None:
+            x = x.contiguous()
+            src = _rows_view(x, d)
+        dst = _rows_view(y, d)
+        ok, need = dst is not None, 0 if dst is None else dst[3]
+        for stride, count in sorted([(dst[1], dst[0]), (dst[2], n)]) if ok else []:
+            if count > 1:
+                ok, need = ok and stride >= need, stride * (count - 1) + need
+        if not ok:
+            raise GvdHipError('reorder_rows: result %d is not made of whole rows of their own (strides %s)' % (i, y.stride()))
+        items.append((x, y, src, dst))
+    if not parent.is_cuda:
+        raise GvdHipError('reorder_rows: non-GPU tensor; there is no CPU fallback')
+    if out is not None:
+        spans = sorted([_extent(y) + (1,) for _, y, _, _ in items] + [_extent(x) + (0,) for x, _, _, _ in items])
+        end, wend = 0, 0
+        for a, b, written in spans:                  # (states may overlap each other; a result may overlap nothing)
+            if a < wend or written and a < end:
+                raise GvdHipError('reorder_rows: a result overlaps a state or another result')
+            end = max(end, b)
+            wend = max(wend, b) if written else wend
+    with torch.cuda.device(dev):
+        for k in range(0, len(items), REORDER_MAX_TENSORS):
+            part = items[k:k + REORDER_MAX_TENSORS]
+            g = ReorderGroup()
+            g.count = len(part)
+            for i, (x, y, (outer, so, sr, row), (_, do, dr, _)) in enumerate(part):
+                t = g.t[i]
+                t.src, t.dst = x.data_ptr(), y.data_ptr()
+                t.outer, t.src_outer, t.dst_outer, t.src_row, t.dst_row, t.row_bytes = outer, so, do, sr, dr, row
+            check(lib().gvd_reorder_rows(C.byref(g), ptr(parent), rows, n, stream_on(dev)), 'gvd_reorder_rows')
+    return results

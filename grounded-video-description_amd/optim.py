@@ -12,7 +12,8 @@ import math
 
 import torch
 
-from .hip import OPT_CHUNK, OPT_MAX_TENSORS, GvdHipError, OptGroup, check, lib, ptr, stream_ptr
+from .hip import (DTYPES, GRAD_CHUNK, GRAD_MAX_TENSORS, OPT_CHUNK, OPT_MAX_TENSORS, GradClip, GradGroup, GvdHipError, OptGroup, check,
+                  lib, ptr, stream_on, stream_ptr)
 
 
 class ClipAdam(torch.optim.Adam):
@@ -139,3 +140,193 @@ class ClipAdam(torch.optim.Adam):
 
     def step(self, closure=None):
         self.step_clipped(None, closure)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The global gradient norm and clipping as operators of their own (csrc/grad_clip.hip), for optimisers other than ClipAdam:
+# fp32, bf16 and fp16 gradients, mixed, clipped in place or written - unscaled - into master gradients of another type.
+# ---------------------------------------------------------------------------------------------------------------------
+def _dense(t):
+    """t's elements fill one stretch of memory, each at a place of its own (in whatever order)."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if s != step:
+            return False
+        step *= n
+    return True
+
+
+def _check_grads(grads, what):
+    """The gradients that have elements; dense float tensors on one GPU."""
+    for i, g in enumerate(grads):
+        if g.dtype not in DTYPES or g.layout != torch.strided:
+            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s %s'
+                              % (what, i, g.layout, g.dtype))
+        if g.device != grads[0].device:
+            raise GvdHipError('%s: gradients on %s and %s' % (what, grads[0].device, g.device))
+    if grads and not grads[0].is_cuda:
+        raise GvdHipError('%s: the gradients are not on the GPU; there is no CPU fallback' % what)
+    return [g for g in grads if g.numel()]
+
+
+def _no_overlap(tensors, what):
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise GvdHipError('%s: two of the tensors to be written share memory' % what)
+
+
+def _grad_groups(grads, out):
+    """Launch arguments of at most GRAD_MAX_TENSORS tensors each; out: the tensors to be written (None: the norm alone)."""
+    groups = []
+    for k in range(0, len(grads), GRAD_MAX_TENSORS):
+        part = grads[k:k + GRAD_MAX_TENSORS]
+        g = GradGroup()
+        g.count = len(part)
+        ns = [t.numel() for t in part]
+        g.src[:len(part)] = [t.data_ptr() for t in part]
+        g.n[:len(part)] = ns
+        g.src_type[:len(part)] = [DTYPES[t.dtype] for t in part]
+        at, firsts = 0, [0]
+        for n in ns:
+            at += -(-n // GRAD_CHUNK)
+            firsts.append(at)
+        g.chunk0[:len(part) + 1] = firsts
+        if out is not None:
+            w = out[k:k + GRAD_MAX_TENSORS]
+            g.dst[:len(part)] = [t.data_ptr() for t in w]
+            g.dst_type[:len(part)] = [DTYPES[t.dtype] for t in w]
+        groups.append(g)
+    return groups
+
+
+def _norm_and_scale(grads, out, max_norm, inv_scale, error_if_nonfinite, what):
+    """grads: live, dense.  The norm (device scalar); out (tensors like grads) = the clipped gradients, None = the norm alone."""
+    dev = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    groups = _grad_groups(grads, out)
+    l = lib()
+    parts = []
+    for g in groups:
+        n = l.gvd_grad_parts(C.byref(g))
+        if n <= 0:
+            raise GvdHipError('%s: the gradients are too large for one call' % what)
+        parts.append(n)
+    partials = torch.empty(sum(parts), dtype=torch.float64, device=dev)
+    c = GradClip(max_norm, inv_scale)
+    with torch.cuda.device(dev):
+        st = stream_on(dev)
+        at = partials.data_ptr()
+        for g, n in zip(groups, parts):
+            check(l.gvd_grad_sumsq(C.byref(g), at, st), 'gvd_grad_sumsq')
+            at += 8 * n
+        if out is None or error_if_nonfinite:
+            check(l.gvd_grad_scale(C.byref(GradGroup()), C.byref(c), ptr(partials), sum(parts), ptr(norm), st), 'gvd_grad_scale')
+            if error_if_nonfinite and not bool(torch.isfinite(norm)):
+                raise RuntimeError('%s: the total norm of the gradients is not finite (%s); they were not clipped' % (what, float(norm)))
+        if out is not None:
+            for i, g in enumerate(groups):
+                check(l.gvd_grad_scale(C.byref(g), C.byref(c), ptr(partials), sum(parts), None if i else ptr(norm), st),
+                      'gvd_grad_scale')
+    return norm
+
+
+def _check_clip(max_norm, inv_scale, what):
+    max_norm, inv_scale = float(max_norm), float(inv_scale)
+    if not max_norm >= 0.0:
+        raise GvdHipError('%s: max_norm must be >= 0, got %r' % (what, max_norm))
+    if not 0.0 < inv_scale < math.inf:
+        raise GvdHipError('%s: inv_scale must be positive and finite, got %r' % (what, inv_scale))
+    return max_norm, inv_scale
+
+
+@torch.no_grad()
+def grad_norm(grads, inv_scale=1.0):
+    """inv_scale * the L2 norm of all elements of all tensors, a float32 scalar on their device (0 for none).  Summed in fp64 in a
+    fixed order.  fp32 / bf16 / fp16 tensors of any strides, on one GPU."""
+    what = 'grad_norm'
+    _, inv_scale = _check_clip(0.0, inv_scale, what)
+    grads = list(grads)
+    live = _check_grads(grads, what)
+    if not live:
+        return torch.zeros((), device=grads[0].device if grads else 'cuda')
+    return _norm_and_scale([g if _dense(g) else g.contiguous() for g in live], None, 0.0, inv_scale, False, what)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=False):
+    """grads * min(1, max_norm / (norm + 1e-6)) * inv_scale, where norm = inv_scale * the L2 norm of them all.
+
+    In place, or into `out` (one tensor per gradient, of its shape, any of the three types: 16-bit gradients of a scaled loss go
+    unscaled and clipped into fp32 master gradients; views of a flat buffer are fine).  Returns the norm before clipping, a
+    float32 scalar on the device; nothing waits for the GPU unless error_if_nonfinite is set, which raises RuntimeError before
+    anything is written if the norm is NaN or infinite.  Otherwise a NaN norm makes every gradient NaN and an infinite one every
+    finite gradient 0, as torch.nn.utils.clip_grad_norm_ does.  One GPU; tensors to be written must not share memory."""
+    what = 'clip_grads'
+    max_norm, inv_scale = _check_clip(max_norm, inv_scale, what)
+    grads = list(grads)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise GvdHipError('%s: %d gradients, %d results' % (what, len(grads), len(out)))
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if o.device != g.device or o.dtype not in DTYPES or o.shape != g.shape:
+                raise GvdHipError('%s: result %d must be a float32 / bfloat16 / float16 tensor %s on %s' % (what, i, tuple(g.shape),
+                                                                                                            g.device))
+        out = [o for o in out if o.numel()]
+    live = _check_grads(grads, what)
+    if not live:
+        return torch.zeros((), device=grads[0].device if grads else 'cuda')
+    if out is None:
+        src = [g if _dense(g) else g.contiguous() for g in live]
+        dst, back = src, [(g, s) for g, s in zip(live, src) if s is not g]
+        for g, _ in back:
+            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+                raise GvdHipError('%s: a gradient of strides %s cannot be clipped in place' % (what, g.stride()))
+    else:
+        # element i of a result belongs to element i of its gradient: same order in memory, or both in row-major order
+        src, dst, back = [], [], []
+        for g, o in zip(live, out):
+            if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+                raise GvdHipError('%s: a result of strides %s cannot be written' % (what, o.stride()))
+            same = g.stride() == o.stride() and _dense(g)
+            src.append(g if same else g.contiguous())
+            dst.append(o if same or o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format))
+            if dst[-1] is not o:
+                back.append((o, dst[-1]))
+    _no_overlap(dst, what)
+    if out is not None:
+        _no_partial_alias(src, dst, what)
+    norm = _norm_and_scale(src, dst, max_norm, inv_scale, error_if_nonfinite, what)
+    for o, d in back:
+        o.copy_(d)
+    written = live if out is None else out
+    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    return norm
+
+
+def _no_partial_alias(src, dst, what):
+    """A result is its own gradient (clipped in place) or shares no memory with any gradient."""
+    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, 0) for i, t in enumerate(src)] +
+                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, 1) for i, t in enumerate(dst)])
+    open_ = []
+    for a, b, i, written in spans:
+        open_ = [s for s in open_ if s[1] > a]
+        for a2, b2, j, w2 in open_:
+            own = i == j and (a, b) == (a2, b2) and src[i].dtype == dst[i].dtype
+            if written != w2 and not own:
+                raise GvdHipError('%s: a result shares memory with a gradient that is not its own' % what)
+        open_.append((a, b, i, written))
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ (main.py:265) on the library's kernels: the gradients of `parameters` (a tensor or an
+    iterable of tensors; those without a gradient are passed over) are scaled in place by min(1, max_norm / (norm + 1e-6)).
+    Returns the norm before clipping.  The L2 norm only."""
+    if float(norm_type) != 2.0:
+        raise GvdHipError('clip_grad_norm_: the L2 norm only (norm_type = 2), got %r' % (norm_type,))
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, error_if_nonfinite=error_if_nonfinite)

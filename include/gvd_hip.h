@@ -35,7 +35,7 @@ typedef struct ihipStream_t* gvd_stream_t; /* == hipStream_t */
 /* library / build identification (also lets tests prove the HIP library, not a fallback, is loaded).
  * GVD_ABI_VERSION changes whenever a struct layout or signature below changes; the Python binding refuses a
  * library whose gvd_abi_version() differs from the version it was written against (hip.ABI_VERSION). */
-#define GVD_ABI_VERSION 20
+#define GVD_ABI_VERSION 21
 const char* gvd_version(void);
 int gvd_abi_version(void);
 
@@ -701,6 +701,96 @@ int gvd_clip_coef(const float* partials, int n, float max_norm, float* out, gvd_
  * for that read first. */
 int gvd_adam_step(const gvd_opt_group* g, const float* clip, const int* skip, int n_skip, float beta1, float beta2,
                   float eps, float weight_decay, gvd_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Token-side operators of training and search, for fp32 and 16-bit tensors (csrc/embedding.hip, grad_clip.hip,
+ * beam_select.hip).  Arithmetic is fp32 or wider; a value is rounded once, where it is stored.
+ * ------------------------------------------------------------------------------------------- */
+#define GVD_F32 0
+#define GVD_BF16 1
+#define GVD_F16 2
+
+/* Embedding lookup: out[i,:] = act(scale * table[tokens[i],:]), i < n.  tokens: int64 (tok64 != 0) or int32, contiguous;
+ * table [vocab, width] (row stride ld), out [n, width] (row stride ldo), both of type dtype, elements of a row contiguous; act: 0
+ * none, 1 ReLU.  A token outside [0, vocab) reads nothing; its row of out is NaN.
+ * Limits: n, vocab <= GVD_EMBEDDING_MAX, width <= 2^20. */
+#define GVD_EMBEDDING_MAX (1 << 25)
+int gvd_embedding_fwd(const void* tokens, int tok64, int64_t n, const void* table, int64_t ld, int64_t vocab, int width, int dtype,
+                      float scale, int act, void* out, int64_t ldo, gvd_stream_t stream);
+
+/* Its gradient: dw[v,:] = scale * act'(scale * table[v,:]) * sum over i with tokens[i] = v of dy[i,:], every row of the
+ * contiguous dw [vocab, width] written once (tokens not met, and row padding_idx, as zeros; -1 = no padding row); tokens
+ * outside [0, vocab) add nothing.  dy [n, width] with row stride ld_dy (0 = one row for all).  table is read for act = 1 only.
+ * Positions are sorted by token and summed in fp32 in a fixed order: no atomics, the same bits at every run.
+ * workspace: gvd_embedding_bwd_workspace_bytes(n, vocab, width) bytes, 16-byte aligned, contents free. */
+size_t gvd_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int width);
+int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const void* dy, int64_t ld_dy, const void* table, int64_t ld,
+                      int64_t vocab, int width, int dtype, float scale, int act, int64_t padding_idx, void* dw, void* workspace,
+                      size_t workspace_bytes, gvd_stream_t stream);
+
+/* Global gradient norm over many tensors, and clipping.  A group holds up to GVD_GRAD_MAX_TENSORS dense tensors of n[t] > 0
+ * elements: src[t] of type src_type[t], for gvd_grad_scale also dst[t] of type dst_type[t] (= src[t]: in place, same type);
+ * chunk0[t] = sum over the tensors before t of ceil(n / gvd_grad_chunk()), chunk0[count] = the total.
+ *   gvd_grad_sumsq    writes gvd_grad_parts(group) doubles to partials: sums of squares of parts of the group
+ *   gvd_grad_scale    norm = inv_scale * sqrt(sum of all n_partials partials, of all groups), *norm_out = norm (nullable),
+ *                     dst = src * min(1, max_norm / (norm + 1e-6)) * inv_scale.  count = 0: only *norm_out is written.
+ * A group that is clipped in place with factor 1 is neither read nor written. */
+#define GVD_GRAD_MAX_TENSORS 120
+#define GVD_GRAD_CHUNK 8192
+typedef struct {
+  const void* src[GVD_GRAD_MAX_TENSORS];
+  void* dst[GVD_GRAD_MAX_TENSORS];
+  int64_t n[GVD_GRAD_MAX_TENSORS];
+  uint32_t chunk0[GVD_GRAD_MAX_TENSORS + 1];
+  uint8_t src_type[GVD_GRAD_MAX_TENSORS];
+  uint8_t dst_type[GVD_GRAD_MAX_TENSORS];
+  int count;
+} gvd_grad_group;
+typedef struct { double max_norm, inv_scale; } gvd_grad_clip;
+
+int gvd_grad_chunk(void);
+int gvd_grad_parts(const gvd_grad_group* g);
+int gvd_grad_sumsq(const gvd_grad_group* g, void* partials, gvd_stream_t stream);
+int gvd_grad_scale(const gvd_grad_group* g, const gvd_grad_clip* c, const void* partials, int n_partials, float* norm_out,
+                   gvd_stream_t stream);
+
+/* Beam search's selection of one step: for each of B samples the W best of the K * V candidates
+ *   cand[q,v] = scores[b,q] + (logits[b*K+q, v] - log sum_v exp(logits[b*K+q, v]))
+ * in descending order, equal ones by q * V + v ascending, computed and compared in fp64 (words of one beam: by their logits).
+ * finished (nullable, u8 [B,K]): an ended beam has scores[b,q] for the word eos and -inf for the others; its logits are not
+ * read.  A beam whose score or log-sum-exp is not finite has -inf for every word.  logits [B*K, V] of type dtype, row stride ld.
+ * Out, [B,W] each: out_scores f32, parent = b*K + q, word, out_finished = finished[b,q] or word == eos (nullable; eos = -1: none).
+ * Limits: K, W <= GVD_BEAM_SELECT_MAX, W <= K * V, B * K <= 65535, V <= 2^28.
+ * workspace: gvd_beam_select_workspace_bytes(B, K, V, W) bytes, 16-byte aligned, contents free. */
+#define GVD_BEAM_SELECT_MAX 32
+typedef struct {
+  const void* logits; int64_t ld; int dtype;
+  int B, K, V, W, eos;
+  const float* scores; const uint8_t* finished;
+  float* out_scores; int64_t* parent; int64_t* word; uint8_t* out_finished;
+  void* workspace; size_t workspace_bytes;
+} gvd_beam_select_args;
+
+size_t gvd_beam_select_workspace_bytes(int B, int K, int V, int W);
+int gvd_beam_select(const gvd_beam_select_args* args, gvd_stream_t stream);
+
+/* Reordering of the beams' states: dst[o, r, :] = src[o, index[r], :] for up to GVD_REORDER_MAX_TENSORS tensors in one launch.
+ * A tensor is [outer, rows, row_bytes] with the byte strides src_outer / src_row and dst_outer / dst_row; index int64
+ * [rows_out], shared by the tensors.  src and dst must not overlap.  An index outside [0, rows_in) reads nothing: its
+ * rows get all bits set (NaN, -1).  `unit` and `tile0` are filled in by the call. */
+#define GVD_REORDER_MAX_TENSORS 16
+typedef struct {
+  const void* src; void* dst;
+  int64_t outer, src_outer, dst_outer, src_row, dst_row, row_bytes;
+  int unit;
+} gvd_reorder_tensor;
+typedef struct {
+  gvd_reorder_tensor t[GVD_REORDER_MAX_TENSORS];
+  int64_t tile0[GVD_REORDER_MAX_TENSORS + 1];
+  int count;
+} gvd_reorder_group;
+
+int gvd_reorder_rows(const gvd_reorder_group* g, const int64_t* index, int64_t rows_in, int64_t rows_out, gvd_stream_t stream);
 
 #ifdef __cplusplus
 }
