@@ -17,7 +17,8 @@ namespace {
 
 constexpr int MAX_BEAMS = GVD_BEAM_SELECT_MAX, MAX_WIDTH = GVD_BEAM_SELECT_MAX;
 constexpr int MAX_PARTS = 64;             // parts of a row: one lane each in the join
-constexpr int LIST = 512;                 // words at or over the threshold that one tile may have before it is ranked the slow way
+constexpr int JOIN_LIST = 256;            // words of all parts of a row
+constexpr int LIST = 192;                 // words a wave collects before it ranks them
 
 typedef unsigned long long u64;
 
@@ -52,148 +53,168 @@ __device__ __forceinline__ u64 wave_max_u64(u64 v) {
   return v;
 }
 
-// One part of one row.  A thread holds IPT logits of a tile.  Threshold: among the 64 lanes' maxima of a wave, the W-th largest
-// is at most the W-th largest logit of the tile, so only logits at or over (the largest such value of the four waves) can be among
-// the best W: usually a few more than W.  They are put on a list and ranked against each other.
+__device__ __forceinline__ int lanes_below(u64 mask, int lane) { return __popcll(mask & ((1ull << lane) - 1ull)); }
+
+// the best W of the n words on a wave's list, in order, to its front: every word counts those before it
+__device__ __forceinline__ void rank_list(u64* list, int n, int W, int lane) {
+  u64 k[LIST / 64];
+  int r[LIST / 64];
+#pragma unroll
+  for (int i = 0; i < LIST / 64; ++i) { k[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0; r[i] = 0; }
+  if (n <= 64) {
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r[0] += list[j] > k[0];
+  } else {
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const u64 o = list[j];
+#pragma unroll
+      for (int i = 0; i < LIST / 64; ++i) r[i] += o > k[i];
+    }
+  }
+  wave_lds_fence();
+  if (lane < W) list[lane] = 0;
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < LIST / 64; ++i)
+    if (k[i] && r[i] < W) list[r[i]] = k[i];
+  wave_lds_fence();
+}
+
+// One wave per part of a row: 64 * IPT logits at a time, the next ones on their way meanwhile.  Every lane has a running maximum
+// and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a bound from
+// the first tile: with the lanes in W or more equal groups, the smallest of the groups' maxima is reached by W words.  The list is
+// ranked, and the floor raised, when it is full; logits of any order and equality only make that more frequent.
 template <typename T, int IPT>
 __global__ __launch_bounds__(256) void beam_part_kernel(const SelectArgs a) {
-  constexpr int N = IPT < 16 / (int)sizeof(T) ? IPT : 16 / (int)sizeof(T);
-  constexpr int TILE = 256 * IPT;
-  __shared__ u64 s_list[LIST];
-  __shared__ u64 s_best[MAX_WIDTH];
-  __shared__ float s_max[4];
-  __shared__ unsigned s_thr[4];
-  __shared__ u64 s_top[4];
-  __shared__ double s_sum[4];
-  __shared__ int s_n;
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int row = blockIdx.y;
-  if (a.finished && a.finished[row]) return;
-  if (!(fabsf(a.scores[row]) < INFINITY)) return;
+  constexpr int N = 16 / (int)sizeof(T), VECS = IPT / N, TILE = 64 * IPT;
+  typedef typename GvdVec<T, N>::type Vec;
+  typedef typename GvdVec<T, N>::loose Loose;
+  __shared__ u64 s_list[4][LIST];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int part = blockIdx.x * 4 + wave, row = blockIdx.y;
+  if (part >= a.parts) return;
+  const bool skip = (a.finished && a.finished[row]) || !(fabsf(a.scores[row]) < INFINITY);
   const int W = a.W, V = a.V;
   const T* x = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld;
+  u64* list = s_list[wave];
+  if (lane < W) list[lane] = 0;
+  int n = W;                               // words on the list, the best W of before in front
+  u64 floor = 0;
   double sum = 0.0;
   float top = -INFINITY;
-  if (tid < MAX_WIDTH) s_best[tid] = 0;
-  if (tid == 0) s_n = 0;
-  const int64_t first = (int64_t)blockIdx.x * a.tiles_per_part;
-  for (int t = 0; t < a.tiles_per_part; ++t) {
-    const int64_t v0 = (first + t) * TILE;
-    if (v0 >= V) break;
+  const int64_t first = (int64_t)part * a.tiles_per_part * TILE;
+  const int64_t end = first + (int64_t)a.tiles_per_part * TILE < V ? first + (int64_t)a.tiles_per_part * TILE : V;
+  Vec next[VECS];
+  const auto fetch = [&](int64_t v0) {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int64_t at = v0 + (i * 64 + lane) * N;
+      if (at + N <= V) next[i] = *reinterpret_cast<const Loose*>(x + at);
+      else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) next[i][k] = at + k < V ? x[at + k] : (T)-INFINITY;
+      }
+    }
+  };
+  if (skip) return;
+  fetch(first);
+  for (int64_t v0 = first; v0 < end; v0 += TILE) {
     float v[IPT];
     float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < IPT / N; ++i) {
-      const int64_t at = v0 + (int64_t)(i * 256 + tid) * N;
-      float y[N];
-      if (at + N <= V) gvd_load<T, N>(x + at, y);
-      else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) y[k] = at + k < V ? (float)x[at + k] : -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < N; ++k) { v[i * N + k] = y[k]; mx = fmaxf(mx, y[k]); }
-    }
-    // W-th largest of the lanes' maxima, bit by bit
-    const unsigned mine = order_bits(mx);
-    unsigned thr = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned c = thr | (1u << bit);
-      if (__popcll(__ballot(mine >= c)) >= W) thr = c;
-    }
-    mx = wave_max(mx);
-    if ((tid & 63) == 0) { s_max[wave] = mx; s_thr[wave] = thr; }
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    thr = max(max(s_thr[0], s_thr[1]), max(s_thr[2], s_thr[3]));
-    thr = max(thr, (unsigned)(s_best[W - 1] >> 32));
+    for (int i = 0; i < IPT; ++i) { v[i] = (float)next[i / N][i % N]; mx = fmaxf(mx, v[i]); }
+    if (v0 + TILE < end) fetch(v0 + TILE);
+    // softmax: terms 2^((x - top) log2 e) on v_exp_f32; nothing but -inf so far: every term is 0
     const float was = top;
     top = fmaxf(top, mx);
-    const float ref = top > -INFINITY ? top : 0.f;           // (nothing but -inf so far: every term is exp(-inf) = 0)
-    float part = 0.f;
+    const float ref = top > -INFINITY ? top : 0.f;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) part += expf(v[i] - ref);
-    sum = sum * (double)expf(was - ref) + (double)part;
-    // the list: the best of the tiles before, then this tile's words at or over the threshold
+    for (int i = 0; i < IPT; ++i) s[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * 1.44269504088896341f);
+    sum = sum * (double)__builtin_amdgcn_exp2f((was - ref) * 1.44269504088896341f) + (double)((s[0] + s[1]) + (s[2] + s[3]));
+    const unsigned ub = order_bits(mx);
+    if (v0 == first) {
+      unsigned g = ub;
+      int off = 1;
+      for (; off * 2 * W <= 64; off *= 2) g = max(g, (unsigned)__shfl_xor((int)g, off, GVD_WAVE));
+      for (; off < 64; off *= 2) g = min(g, (unsigned)__shfl_xor((int)g, off, GVD_WAVE));
+      floor = (u64)g << 32;
+    }
+    if (!__ballot(ub >= (unsigned)(floor >> 32))) continue;
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
-      const int64_t at = v0 + (int64_t)((i / N) * 256 + tid) * N + i % N;
-      const unsigned u = order_bits(v[i]);
-      if (u >= thr && at < V) {
-        const int k = atomicAdd(&s_n, 1);
-        if (k < LIST - MAX_WIDTH) s_list[MAX_WIDTH + k] = make_key(u, (int)at);
-      }
-    }
-    if (tid < MAX_WIDTH) s_list[tid] = s_best[tid];
-    __syncthreads();
-    const int n = s_n;
-    if (n <= LIST - MAX_WIDTH) {
-      for (int i = tid; i < MAX_WIDTH + n; i += 256) {
-        const u64 k = s_list[i];
-        int rank = 0;
-        for (int j = 0; j < MAX_WIDTH + n; ++j) rank += s_list[j] > k;
-        if (k && rank < W) s_best[rank] = k;
-      }
-    } else {
-      // more words at the threshold than the list holds (equal logits): W times the best of what is left
-      u64 last = ~0ull;
-      for (int r = 0; r < W; ++r) {
-        u64 k = 0;
-        if (tid < MAX_WIDTH && s_list[tid] < last) k = s_list[tid];
-#pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-          const int64_t at = v0 + (int64_t)((i / N) * 256 + tid) * N + i % N;
-          const u64 c = at < V ? make_key(order_bits(v[i]), (int)at) : 0;
-          if (c < last && c > k) k = c;
+      const int64_t at = v0 + ((i / N) * 64 + lane) * N + i % N;
+      const u64 key = make_key(order_bits(v[i]), (int)at);
+      const bool hit = key >= floor && at < V;
+      const u64 hits = __ballot(hit);
+      if (hits) {
+        const int c = __popcll(hits);
+        if (n + c > LIST) {
+          wave_lds_fence();
+          rank_list(list, n, W, lane);
+          n = W;
+          floor = list[W - 1] > floor ? list[W - 1] : floor;
         }
-        k = wave_max_u64(k);
-        if ((tid & 63) == 0) s_top[wave] = k;
-        __syncthreads();
-        k = s_top[0];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) k = s_top[w] > k ? s_top[w] : k;
-        if (tid == 0) s_best[r] = k;
-        last = k;
-        __syncthreads();
+        if (hit) list[n + lanes_below(hits, lane)] = key;
+        n += c;
       }
     }
-    __syncthreads();
-    if (tid == 0) s_n = 0;
-    __syncthreads();
+    if (v0 + TILE < end && n > W) {
+      wave_lds_fence();
+      rank_list(list, n, W, lane);
+      n = W;
+      floor = list[W - 1] > floor ? list[W - 1] : floor;
+    }
   }
+  wave_lds_fence();
+  if (n > W) rank_list(list, n, W, lane);
+  // the lanes' sums, each to its own maximum, into one (NaN and +inf go through to the join, which drops the beam)
+  const float all = wave_max(top);
+  sum = sum != 0.0 ? sum * exp((double)top - (double)all) : 0.0;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, GVD_WAVE);
-  if ((tid & 63) == 0) s_sum[wave] = sum;
-  __syncthreads();
-  const int64_t rec = (int64_t)row * a.parts + blockIdx.x;
-  if (tid == 0) a.stat[rec] = make_double2((double)top, (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
-  if (tid < W) a.best[rec * W + tid] = s_best[tid];
+  const int64_t rec = (int64_t)row * a.parts + part;
+  if (lane == 0) a.stat[rec] = make_double2((double)all, sum);
+  if (lane < W) a.best[rec * W + lane] = list[lane];
 }
 
-// One workgroup per sample, one wave per beam (and the beams 16 further on): a lane holds the head of one part's list, the
-// wave takes the best head W times.  Then the first wave does the same over the beams' lists.
+// One workgroup per sample, one wave per beam (and the beams 16 further on): the words of the row's parts at or over the best
+// W-th word of a part are put on a list and ranked.  Then all waves do the same with the candidates of the beams.
 __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
-  __shared__ double s_score[MAX_BEAMS][MAX_WIDTH];
-  __shared__ int s_word[MAX_BEAMS][MAX_WIDTH];
+  __shared__ double s_score[MAX_BEAMS * MAX_WIDTH];
+  __shared__ int s_word[MAX_BEAMS * MAX_WIDTH];
+  __shared__ u64 s_list[16][JOIN_LIST];
+  __shared__ int s_n;
   const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int K = a.K, W = a.W, V = a.V;
+  if (threadIdx.x == 0) s_n = 0;
   for (int q = wave; q < K; q += waves) {
     const int row = b * K + q;
+    double* score_q = s_score + q * W;
+    int* word_q = s_word + q * W;
     const float score = a.scores[row];
     const bool over = a.finished && a.finished[row];
     bool live = fabsf(score) < INFINITY;
     if (live && over) {
       if (lane < W) {
         const int w = lane == 0 ? a.eos : lane - 1 < a.eos ? lane - 1 : lane;
-        s_score[q][lane] = lane == 0 ? (double)score : -INFINITY;
-        s_word[q][lane] = w < V ? w : -1;
+        score_q[lane] = lane == 0 ? (double)score : -INFINITY;
+        word_q[lane] = w < V ? w : -1;
       }
       continue;
     }
     double lse = 0.0;
+    u64 mine[JOIN_LIST / 64];
+    u64 floor = 0;
+    const int total = a.parts * W;
     if (live) {
-      const int64_t rec = (int64_t)row * a.parts + lane;
-      const double2 st = lane < a.parts ? a.stat[rec] : make_double2(-INFINITY, 0.0);
+      const int64_t rec = (int64_t)row * a.parts;
+      const double2 st = lane < a.parts ? a.stat[rec + lane] : make_double2(-INFINITY, 0.0);
+      const u64* list = a.best + rec * W;
+      floor = lane < a.parts ? list[lane * W + W - 1] : 0;
+#pragma unroll
+      for (int i = 0; i < JOIN_LIST / 64; ++i) mine[i] = lane + 64 * i < total ? list[lane + 64 * i] : 0;
       double m = st.x;
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) m = fmax(m, __shfl_xor(m, off, GVD_WAVE));
@@ -205,70 +226,90 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
     }
     if (!live) {
       if (lane < W) {
-        s_score[q][lane] = -INFINITY;
-        s_word[q][lane] = lane < V ? lane : -1;
+        score_q[lane] = -INFINITY;
+        word_q[lane] = lane < V ? lane : -1;
       }
       continue;
     }
-    const u64* list = a.best + ((int64_t)row * a.parts + lane) * W;
-    int at = 0;
-    u64 head = lane < a.parts ? list[0] : 0;
-    for (int r = 0; r < W; ++r) {
-      const u64 k = wave_max_u64(head);
-      if (lane == 0) {
-        s_score[q][r] = (double)score + ((double)from_order_bits((unsigned)(k >> 32)) - lse);
-        s_word[q][r] = k ? key_word(k) : -1;
-      }
-      if (k && head == k) head = ++at < W ? list[at] : 0;
+    floor = wave_max_u64(floor);
+    u64* list = s_list[wave];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < JOIN_LIST / 64; ++i) {
+      if (64 * i >= total) break;
+      const bool keep = mine[i] && mine[i] >= floor;
+      const u64 hits = __ballot(keep);
+      if (keep) list[n + lanes_below(hits, lane)] = mine[i];
+      n += __popcll(hits);
     }
+    if (lane < W) { score_q[lane] = -INFINITY; word_q[lane] = -1; }
+    wave_lds_fence();
+    for (int i = lane; i < n; i += 64) {
+      const u64 k = list[i];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) r += list[j] > k;
+      if (r < W) {
+        score_q[r] = (double)score + ((double)from_order_bits((unsigned)(k >> 32)) - lse);
+        word_q[r] = key_word(k);
+      }
+    }
+    wave_lds_fence();
   }
   __syncthreads();
-  if (wave) return;
-  int at = 0, my_beam = 0, my_word = 0;
-  double my_score = 0.0;
-  for (int r = 0; r < W; ++r) {
-    const bool have = lane < K && at < W && s_word[lane][at] >= 0;
-    double sc = have ? s_score[lane][at] : -INFINITY;
-    int who = have ? lane : 64 + lane;                       // (no candidate left: after every lane that has one)
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const double os = __shfl_xor(sc, off, GVD_WAVE);
-      const int ow = __shfl_xor(who, off, GVD_WAVE);
-      if (os > sc || (os == sc && ow < who)) { sc = os; who = ow; }
+  // candidates by (score descending, place in the lists ascending): a beam's list is in order already, and beams go up
+  double floor = -INFINITY;
+  for (int q = 0; q < K; ++q)
+    if (s_word[q * W + W - 1] >= 0) floor = fmax(floor, s_score[q * W + W - 1]);
+  double* kept_score = reinterpret_cast<double*>(&s_list[0][0]);
+  int* kept = reinterpret_cast<int*>(kept_score + MAX_BEAMS * MAX_WIDTH);
+  for (int e = threadIdx.x; e < K * W; e += blockDim.x)
+    if (s_word[e] >= 0 && s_score[e] >= floor) {
+      const int at = atomicAdd(&s_n, 1);
+      kept[at] = e;
+      kept_score[at] = s_score[e];
     }
-    const int beam = who & 63;
-    const int w = s_word[beam][__shfl(at, beam, GVD_WAVE)];
-    if (lane == r) { my_score = sc; my_beam = beam; my_word = w; }
-    if (lane == beam) ++at;
-  }
-  if (lane < W) {
-    const int64_t o = (int64_t)b * W + lane;
-    a.out_scores[o] = (float)my_score;
-    a.parent[o] = (int64_t)b * K + my_beam;
-    a.word[o] = my_word;
-    if (a.out_finished) a.out_finished[o] = my_word == a.eos || (a.finished && a.finished[b * K + my_beam]);
+  __syncthreads();
+  const int n = s_n;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int e = kept[i];
+    const double sc = kept_score[i];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r += kept_score[j] > sc || (kept_score[j] == sc && kept[j] < e);
+    if (r < W) {
+      const int64_t to = (int64_t)b * W + r;
+      const int q = e / W, w = s_word[e];
+      a.out_scores[to] = (float)sc;
+      a.parent[to] = (int64_t)b * K + q;
+      a.word[to] = w;
+      if (a.out_finished) a.out_finished[to] = w == a.eos || (a.finished && a.finished[b * K + q]);
+    }
   }
 }
 
-// words of one workgroup's tile, parts of a row
+// logits of one lane and tile, parts (waves) of a row, tiles of a part
 struct SelectShape { int ipt, parts, tiles_per_part; };
 
-SelectShape select_shape(int64_t rows, int V) {
+SelectShape select_shape(int64_t rows, int V, int W, int dtype) {
   SelectShape s;
+  const int least = dtype == GVD_F32 ? 4 : 8;
+  int64_t most = MAX_PARTS < JOIN_LIST / W ? MAX_PARTS : JOIN_LIST / W;
+  if (most > 4096 / rows) most = 4096 / rows > 1 ? 4096 / rows : 1;
   s.ipt = 32;
-  while (s.ipt > 4 && (rows * ((V + 256 * s.ipt - 1) / (256 * s.ipt)) < 512 || 128 * s.ipt >= V)) s.ipt /= 2;
-  const int tiles = (V + 256 * s.ipt - 1) / (256 * s.ipt);
-  s.tiles_per_part = (tiles + MAX_PARTS - 1) / MAX_PARTS;
+  while (s.ipt > least && ((V + 64 * s.ipt - 1) / (64 * s.ipt) < most || 32 * s.ipt >= V)) s.ipt /= 2;
+  const int tiles = (V + 64 * s.ipt - 1) / (64 * s.ipt);
+  s.tiles_per_part = (int)((tiles + most - 1) / most);
   s.parts = (tiles + s.tiles_per_part - 1) / s.tiles_per_part;
   return s;
 }
 
 template <typename T> void launch_parts(const SelectArgs& a, int ipt, hipStream_t st) {
-  const dim3 grid((unsigned)a.parts, (unsigned)(a.B * a.K));
+  const dim3 grid((unsigned)((a.parts + 3) / 4), (unsigned)(a.B * a.K));
   if (ipt == 32) hipLaunchKernelGGL((beam_part_kernel<T, 32>), grid, dim3(256), 0, st, a);
   else if (ipt == 16) hipLaunchKernelGGL((beam_part_kernel<T, 16>), grid, dim3(256), 0, st, a);
-  else if (ipt == 8) hipLaunchKernelGGL((beam_part_kernel<T, 8>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((beam_part_kernel<T, 4>), grid, dim3(256), 0, st, a);
+  else if (ipt == 8 || sizeof(T) == 2) hipLaunchKernelGGL((beam_part_kernel<T, 8>), grid, dim3(256), 0, st, a);
+  else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((beam_part_kernel<T, 4>), grid, dim3(256), 0, st, a);
 }
 
 bool bad_select_shape(int B, int K, int V, int W) {
@@ -293,22 +334,35 @@ template <int BYTES>
 __device__ void reorder_tile(const gvd_reorder_tensor& t, const int64_t* __restrict__ index, int64_t rows_in, int64_t rows_out,
                              int64_t tile) {
   typedef typename Unit<BYTES>::type U;
-  const int64_t per_row = (t.row_bytes + BYTES - 1) / BYTES, total = t.outer * rows_out * per_row;
+  const int64_t per_row = (t.row_bytes + BYTES - 1) / BYTES;
   const char* src[4];
   char* dst[4];
-  int live = 0;
+  const auto place = [&](int u, int64_t o, int64_t r, int64_t unit) {
+    int64_t off = unit * BYTES;
+    if (off + BYTES > t.row_bytes) off = t.row_bytes - BYTES;
+    const int64_t from = index[r];
+    dst[u] = reinterpret_cast<char*>(t.dst) + o * t.dst_outer + r * t.dst_row + off;
+    src[u] = from >= 0 && from < rows_in ? reinterpret_cast<const char*>(t.src) + o * t.src_outer + from * t.src_row + off : nullptr;
+  };
+  if (per_row >= UNITS) {                 // a tile lies in one row (the host counts tiles the same way)
+    const int64_t tiles = (per_row + UNITS - 1) / UNITS;
+    const int64_t row = tile / tiles, o = row / rows_out;
+    const int64_t unit0 = (tile - row * tiles) * UNITS + threadIdx.x;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = tile * UNITS + u * 256 + threadIdx.x;
-    src[u] = nullptr; dst[u] = nullptr;
-    if (i < total) {
-      const int64_t row = i / per_row, o = row / rows_out, r = row - o * rows_out;
-      int64_t off = (i - row * per_row) * BYTES;
-      if (off + BYTES > t.row_bytes) off = t.row_bytes - BYTES;
-      const int64_t from = index[r];
-      dst[u] = reinterpret_cast<char*>(t.dst) + o * t.dst_outer + r * t.dst_row + off;
-      if (from >= 0 && from < rows_in) src[u] = reinterpret_cast<const char*>(t.src) + o * t.src_outer + from * t.src_row + off;
-      live = u + 1;
+    for (int u = 0; u < 4; ++u) {
+      dst[u] = nullptr; src[u] = nullptr;
+      if (unit0 + 256 * u < per_row) place(u, o, row - o * rows_out, unit0 + 256 * u);
+    }
+  } else {                                // (fewer than 2^31 units: 32-bit divisions)
+    const unsigned total = (unsigned)(t.outer * rows_out * per_row), pr = (unsigned)per_row, ro = (unsigned)rows_out;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned i = (unsigned)tile * UNITS + u * 256 + threadIdx.x;
+      dst[u] = nullptr; src[u] = nullptr;
+      if (i < total) {
+        const unsigned row = i / pr, o = row / ro;
+        place(u, o, row - o * ro, i - row * pr);
+      }
     }
   }
   U x[4];
@@ -319,7 +373,7 @@ __device__ void reorder_tile(const gvd_reorder_tensor& t, const int64_t* __restr
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (u < live) *reinterpret_cast<U*>(dst[u]) = x[u];
+    if (dst[u]) *reinterpret_cast<U*>(dst[u]) = x[u];
 }
 
 __global__ __launch_bounds__(256) void reorder_rows_kernel(const gvd_reorder_group g, const int64_t* __restrict__ index,
@@ -342,8 +396,12 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(const gvd_reorder_gro
 extern "C" size_t gvd_beam_select_workspace_bytes(int B, int K, int V, int W) {
   if (bad_select_shape(B, K, V, W)) return 0;
   const int64_t rows = (int64_t)B * K;
-  const SelectShape s = select_shape(rows, V);
-  return (size_t)(rows * s.parts * (16 + 8 * (int64_t)W));
+  int64_t most = 0;                        // (of the two shapes: the type is not among the arguments)
+  for (int dtype : {GVD_F32, GVD_BF16}) {
+    const int64_t parts = select_shape(rows, V, W, dtype).parts;
+    most = parts > most ? parts : most;
+  }
+  return (size_t)(rows * most * (16 + 8 * (int64_t)W));
 }
 
 extern "C" int gvd_beam_select(const gvd_beam_select_args* g, gvd_stream_t stream) {
@@ -352,7 +410,7 @@ extern "C" int gvd_beam_select(const gvd_beam_select_args* g, gvd_stream_t strea
       (g->finished && g->eos < 0) || g->workspace_bytes < gvd_beam_select_workspace_bytes(g->B, g->K, g->V, g->W))
     return GVD_EINVAL;
   const int64_t rows = (int64_t)g->B * g->K;
-  const SelectShape s = select_shape(rows, g->V);
+  const SelectShape s = select_shape(rows, g->V, g->W, g->dtype);
   SelectArgs a = {};
   a.logits = g->logits; a.ld = g->ld;
   a.scores = g->scores; a.finished = g->finished;
@@ -386,11 +444,13 @@ extern "C" int gvd_reorder_rows(const gvd_reorder_group* group, const int64_t* i
     while (t.unit > 1 && (t.row_bytes < t.unit || (t.row_bytes < 16 && t.row_bytes % t.unit))) t.unit /= 2;
     g.tile0[i] = tiles;
     const int64_t per_row = (t.row_bytes + t.unit - 1) / t.unit;
-    if (per_row > (1ll << 33) / (t.outer * rows_out)) return GVD_EINVAL;     // (a launch holds fewer than 2^32 threads)
-    tiles += (t.outer * rows_out * per_row + UNITS - 1) / UNITS;
+    if (t.outer > (1ll << 33) / rows_out || per_row > (1ll << 33) / (t.outer * rows_out)) return GVD_EINVAL;
+    if (per_row >= UNITS) tiles += t.outer * rows_out * ((per_row + UNITS - 1) / UNITS);
+    else if (t.outer * rows_out * per_row >= 0x7fffffffll) return GVD_EINVAL;
+    else tiles += (t.outer * rows_out * per_row + UNITS - 1) / UNITS;
   }
   g.tile0[g.count] = tiles;
-  if (tiles > (1ll << 23)) return GVD_EINVAL;
+  if (tiles > (1ll << 23)) return GVD_EINVAL;                   // (a launch holds fewer than 2^32 threads)
   hipLaunchKernelGGL(reorder_rows_kernel, dim3((unsigned)tiles), dim3(256), 0, gvd_s(stream), g, index, rows_in, rows_out);
   GVD_CHECK_LAUNCH();
   return 0;

@@ -48,4 +48,11 @@ template <typename T, int N> __device__ __forceinline__ void gvd_store_part(T* p
     if (k < left) p[k] = (T)v[k];
 }
 
+// LDS accesses of the lanes of one wave before it happen before those after it
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 static inline int gvd_dtype_bytes(int dtype) { return dtype == GVD_F32 ? 4 : (dtype == GVD_BF16 || dtype == GVD_F16) ? 2 : 0; }

@@ -18,33 +18,47 @@ __device__ __forceinline__ unsigned token_key(const void* tok, int tok64, int64_
   return t < 0 || t >= (int64_t)vocab || t == pad ? vocab : (unsigned)t;
 }
 
+__device__ __forceinline__ unsigned wave_id() {
+  return __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));          // (workgroups of four waves)
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
-// One wave per row and 64 * N columns.
-template <typename T, int N>
+// One wave per R rows and 64 * N columns (a slice); the R tokens, then the R rows, are on their way together.  Waves next to each
+// other take the slices of the same rows, so that a row is one stretch of memory traffic.
+template <typename T, int N, int R>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int tok64, int64_t n, const T* __restrict__ table,
                                                             int64_t ld, unsigned vocab, int width, float scale, int act,
-                                                            T* __restrict__ out, int64_t ldo) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= n) return;
-  const int col = (blockIdx.y * 64 + (threadIdx.x & 63)) * N;
-  if (col >= width) return;
-  const unsigned v = token_key(tok, tok64, row, vocab, -1);
+                                                            T* __restrict__ out, int64_t ldo, unsigned slices) {
+  const unsigned id = wave_id(), unit = id / slices;
+  const int64_t row0 = (int64_t)unit * R;
+  const int col = ((int)(id - unit * slices) * 64 + (threadIdx.x & 63)) * N;
+  if (row0 >= n || col >= width) return;
   const int left = width - col;
-  float x[N];
-  if (v == vocab) {                       // a token outside the table: nothing is read, the row is NaN
+  unsigned v[R];
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = __builtin_nanf("");
-  } else {
-    const T* w = table + (int64_t)v * ld + col;
-    if (left >= N) gvd_load<T, N>(w, x); else gvd_load_part<T, N>(w, left, x);
+  for (int r = 0; r < R; ++r) v[r] = row0 + r < n ? token_key(tok, tok64, row0 + r, vocab, -1) : vocab;
+  float x[R][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k] *= scale;
-      if (act) x[k] = act_relu(x[k]);
+  for (int r = 0; r < R; ++r) {
+    if (v[r] == vocab) {                  // a token outside the table: nothing is read, the row is NaN
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[r][k] = __builtin_nanf("");
+    } else {
+      const T* w = table + (int64_t)v[r] * ld + col;
+      if (left >= N) gvd_load<T, N>(w, x[r]); else gvd_load_part<T, N>(w, left, x[r]);
     }
   }
-  T* o = out + row * ldo + col;
-  if (left >= N) gvd_store<T, N>(o, x); else gvd_store_part<T, N>(o, left, x);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row0 + r >= n) break;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[r][k] *= scale;
+      if (act) x[r][k] = act_relu(x[r][k]);
+    }
+    T* o = out + (row0 + r) * ldo + col;
+    if (left >= N) gvd_store<T, N>(o, x[r]); else gvd_store_part<T, N>(o, left, x[r]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------- positions sorted by token
@@ -55,15 +69,30 @@ constexpr int RANK_THREADS = 1024;
 
 __global__ __launch_bounds__(RANK_THREADS) void token_rank_kernel(const void* tok, int tok64, int n, unsigned vocab, int64_t pad,
                                                                   unsigned* __restrict__ skey, unsigned* __restrict__ spos) {
-  __shared__ unsigned s_key[RANK_MAX];
+  __shared__ __attribute__((aligned(16))) unsigned s_key[RANK_MAX];
   __shared__ int s_cnt[16][64];
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int i = tid; i < n; i += RANK_THREADS) s_key[i] = token_key(tok, tok64, i, vocab, pad);
+  const int blocks = (n + 63) >> 6;                            // blocks of 64 keys
+  for (int i = tid; i < 64 * blocks; i += RANK_THREADS) s_key[i] = i < n ? token_key(tok, tok64, i, vocab, pad) : 0xffffffffu;
   __syncthreads();
-  const int i = blockIdx.x * 64 + lane;
-  const unsigned key = i < n ? s_key[i] : 0;
+  const int mine = blockIdx.x, i = mine * 64 + lane;
+  const unsigned key = s_key[i];
+  // blocks before this one count equal keys too (key < mine + 1), blocks behind it only smaller ones
   int c = 0;
-  for (int j = wave; j < n; j += 16) c += s_key[j] < key || (s_key[j] == key && j < i);
+  for (int b = wave; b < blocks; b += 16) {
+    const u32x4* k4 = reinterpret_cast<const u32x4*>(s_key + 64 * b);
+    if (b != mine) {
+      const unsigned than = b < mine ? key + 1 : key;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const u32x4 k = k4[j];
+        c += (k[0] < than) + (k[1] < than) + (k[2] < than) + (k[3] < than);
+      }
+    } else {
+      for (int j = 0; j < 64; ++j) c += s_key[64 * b + j] < (j < lane ? key + 1 : key);
+    }
+  }
   s_cnt[wave][lane] = c;
   __syncthreads();
   if (wave == 0 && i < n) {
@@ -82,7 +111,7 @@ __global__ __launch_bounds__(RANK_THREADS) void token_rank_kernel(const void* to
 constexpr int SORT_BLOCKS = 128;
 constexpr int SORT_BITS = 9;
 constexpr int SORT_DIGITS = 1 << SORT_BITS;
-constexpr int SORT_TILE = 2048;
+constexpr int SORT_TILE = 1024;
 
 struct SortPass {
   const void* tok; int tok64; unsigned vocab; int64_t pad;       // first pass: keys from the tokens, positions 0, 1, ...
@@ -92,13 +121,6 @@ struct SortPass {
   int64_t n, per;                                                // positions; positions of one workgroup
   int shift, bits;
 };
-
-// LDS accesses of the lanes of one wave before it happen before those after it
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 __device__ __forceinline__ unsigned sort_key(const SortPass& p, int64_t i) {
   return p.tok ? token_key(p.tok, p.tok64, i, p.vocab, p.pad) : p.key_in[i];
@@ -118,25 +140,27 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const SortPass p) {
 __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
   __shared__ unsigned s_next[SORT_DIGITS];                   // where the next position of this digit goes
   __shared__ unsigned s_wave[4][SORT_DIGITS];
-  __shared__ unsigned s_sum[256];
+  __shared__ unsigned s_sum[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const unsigned mask = (1u << p.bits) - 1;
   // digits 2 tid, 2 tid + 1: their counts before this part, and in all
   unsigned before[2] = {0, 0}, all[2] = {0, 0};
+#pragma unroll 8
   for (unsigned b = 0; b < gridDim.x; ++b) {
     const uint2 h = *reinterpret_cast<const uint2*>(p.hist + (int64_t)b * SORT_DIGITS + 2 * tid);
     all[0] += h.x; all[1] += h.y;
     if (b < blockIdx.x) { before[0] += h.x; before[1] += h.y; }
   }
-  s_sum[tid] = all[0] + all[1];
-  __syncthreads();
-  for (int off = 1; off < 256; off <<= 1) {
-    const unsigned add = tid >= off ? s_sum[tid - off] : 0;
-    __syncthreads();
-    s_sum[tid] += add;
-    __syncthreads();
+  unsigned upto = all[0] + all[1];
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const unsigned add = __shfl_up(upto, off, GVD_WAVE);
+    if (lane >= off) upto += add;
   }
-  const unsigned base = s_sum[tid] - (all[0] + all[1]);
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+  unsigned base = upto - (all[0] + all[1]);
+  for (int w = 0; w < wave; ++w) base += s_sum[w];
   s_next[2 * tid] = base + before[0];
   s_next[2 * tid + 1] = base + all[0] + before[1];
   const int64_t i0 = (int64_t)blockIdx.x * p.per, i1 = i0 + p.per < p.n ? i0 + p.per : p.n;
@@ -183,64 +207,113 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 }
 
 // ------------------------------------------------------------------------------------------------------- sums by token
-// A token that fills whole groups of GROUP sorted positions (64; and 64 of those groups) has them summed beforehand, one
-// workgroup per group, so that no owner of a row adds up more than a few hundred rows whatever the tokens are.
-constexpr int GROUP = 64;
+// A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one wave
+// per group, so that no owner of a row adds up more than a few hundred rows whatever the tokens are.
+constexpr int GROUP = 32;
+constexpr int64_t LEVEL2_FROM = 4096;     // positions from which the second level pays for its launch
 
 struct SumArgs {
   const unsigned* skey; const unsigned* spos; int64_t n;
   const void* dy; int64_t ld;
-  float* part1; float* part2;             // fp32 [n / 64][width], [n / 4096][width]
+  float* part1; float* part2;             // fp32 [n / GROUP][width], [n / GROUP^2][width]
   const void* table; int64_t ldt;         // for act'
   void* dw;
   unsigned vocab; int width; float scale; int act;
+  unsigned slices; int stretch;
 };
 
-template <typename T, int N> __device__ __forceinline__ void add_row(const T* p, int left, float (&s)[N]) {
-  float x[N];
-  if (left >= N) gvd_load<T, N>(p, x); else gvd_load_part<T, N>(p, left, x);
+// A lane's columns of a row: N of them, the last lane of a row fewer, the lanes behind it none.
+template <typename T, int N> struct Columns {
+  int col, left;
+  typedef typename GvdVec<T, N>::type Raw;       // (as loaded: rows in flight cost half the registers in 16-bit types)
+  __device__ __forceinline__ Raw fetch(const T* row) const {
+    if (left >= N) return *reinterpret_cast<const typename GvdVec<T, N>::loose*>(row + col);
+    Raw x;
 #pragma unroll
-  for (int k = 0; k < N; ++k) s[k] += x[k];
+    for (int k = 0; k < N; ++k) x[k] = k < left ? row[col + k] : (T)0;
+    return x;
+  }
+  __device__ __forceinline__ void store(T* row, const float (&x)[N]) const {
+    if (left >= N) gvd_store<T, N>(row + col, x); else gvd_store_part<T, N>(row + col, left, x);
+  }
+};
+
+// s += `count` (<= 64) rows of x, in order: row i is the one that lane i names (`which`); FLIGHT bytes of a lane on their way at
+// a time, 16 rows at most
+template <typename T, int N, int FLIGHT>
+__device__ __forceinline__ void add_rows(const T* x, int64_t ld, unsigned which, int count, const Columns<T, N>& c, float (&s)[N]) {
+  constexpr int BATCH = FLIGHT / (int)(sizeof(T) * N) < 16 ? FLIGHT / (int)(sizeof(T) * N) : 16;
+  for (int i = 0; i < count; i += BATCH) {
+    typename Columns<T, N>::Raw r[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (i + k < count) r[k] = c.fetch(x + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, i + k) * ld);
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (i + k < count) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += (float)r[k][e];
+      }
+  }
 }
 
-// s += dy rows of sorted positions [i, e), in order
-template <typename T, int N> __device__ __forceinline__ void add_rows(const SumArgs& a, int64_t i, int64_t e, int col, float (&s)[N]) {
-  const T* dy = reinterpret_cast<const T*>(a.dy) + col;
-  const int left = a.width - col;
-  for (; i < e; ++i) add_row<T, N>(dy + (int64_t)a.spos[i] * a.ld, left, s);
+// s += dy rows of the sorted positions [i, e)
+template <typename T, int N>
+__device__ __forceinline__ void add_positions(const SumArgs& a, int64_t i, int64_t e, int lane, const Columns<T, N>& c, float (&s)[N]) {
+  for (; i < e; i += 64) {
+    const unsigned which = i + lane < e ? a.spos[i + lane] : 0;
+    add_rows<T, N, 128>(reinterpret_cast<const T*>(a.dy), a.ld, which, e - i < 64 ? (int)(e - i) : 64, c, s);
+  }
 }
 
-// level 1: groups of 64 positions of one token; level 2: groups of 64 such groups
+// s += rows [i, e) of partial sums
+template <int N>
+__device__ __forceinline__ void add_partials(const float* part, int width, int64_t i, int64_t e, int lane, const Columns<float, N>& c,
+                                             float (&s)[N]) {
+  for (; i < e; i += 64)
+    add_rows<float, N, 128>(part + i * width, width, (unsigned)lane, e - i < 64 ? (int)(e - i) : 64, c, s);
+}
+
+// level 1: whole groups of 32 positions of a token with 64 positions or more; level 2: whole groups of 32 such groups
 template <typename T, int N, int LEVEL>
 __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
-  const int64_t g = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const unsigned id = wave_id(), g = id / a.slices;
+  const int lane = threadIdx.x & 63;
   constexpr int64_t LEN = LEVEL == 1 ? GROUP : GROUP * GROUP;
-  if ((g + 1) * LEN > a.n) return;
-  const unsigned v = a.skey[g * LEN];
-  if (v >= a.vocab || a.skey[g * LEN + LEN - 1] != v) return;
-  const int col = (blockIdx.y * 64 + (threadIdx.x & 63)) * N;
-  if (col >= a.width) return;
-  const int left = a.width - col;
+  const int64_t i0 = (int64_t)g * LEN;
+  if (i0 + LEN > a.n) return;
+  const int col = ((int)(id - g * a.slices) * 64 + lane) * N;
   float s[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) s[k] = 0.f;
+  const Columns<float, N> cf = {col, a.width - col};
   if constexpr (LEVEL == 1) {
-    add_rows<T, N>(a, g * LEN, (g + 1) * LEN, col, s);
+    // keys of [i0 - 32, i0 + 64): the group, and 32 more of the same on its two sides together - else the token has fewer than 64
+    const int64_t b = i0 - 32 + lane, e = i0 + 32 + lane;
+    const unsigned before = b >= 0 ? a.skey[b] : 0xffffffffu, after = lane < 32 && e < a.n ? a.skey[e] : 0xffffffffu;
+    const unsigned which = a.spos[i0 + (lane & 31)];
+    const unsigned v = __builtin_amdgcn_readlane(before, 32);
+    if (v >= a.vocab || __builtin_amdgcn_readlane(before, 63) != v) return;
+    if (__popcll(__ballot(before == v)) + __popcll(__ballot(after == v)) < 64) return;
+    add_rows<T, N, 256>(reinterpret_cast<const T*>(a.dy), a.ld, which, GROUP, Columns<T, N>{col, a.width - col}, s);
   } else {
-    for (int64_t c = g * GROUP; c < (g + 1) * GROUP; ++c) add_row<float, N>(a.part1 + c * a.width + col, left, s);
+    const unsigned v = a.skey[i0], last = a.skey[i0 + LEN - 1];
+    if (v >= a.vocab || last != v) return;
+    add_rows<float, N, 256>(a.part1 + (int64_t)g * GROUP * a.width, a.width, (unsigned)lane, GROUP, cf, s);
   }
-  float* o = (LEVEL == 1 ? a.part1 : a.part2) + g * a.width + col;
-  if (left >= N) gvd_store<float, N>(o, s); else gvd_store_part<float, N>(o, left, s);
+  cf.store((LEVEL == 1 ? a.part1 : a.part2) + (int64_t)g * a.width, s);
 }
 
-// first sorted position whose key is >= v: 64 lanes look at 64 places at a time
-__device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_t n, unsigned v, int lane) {
-  int64_t lo = 0, len = n;                       // the answer is in [lo, lo + len]
+// first sorted position i in [lo, n) with skey[i] >= v (RISE = 0), or skey[i] + i >= v (RISE = 1): 64 lanes look at 64 places at
+// a time
+template <int RISE>
+__device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_t lo, int64_t n, unsigned v, int lane) {
+  int64_t len = n - lo;                          // the answer is in [lo, lo + len]
   while (len > 0) {
     const int64_t step = (len + 63) >> 6;
     const int64_t at = lo + (int64_t)lane * step;
-    const bool less = at < lo + len && skey[at] < v;
-    const int c = __popcll(__ballot(less));      // (sorted: the first c lanes)
+    const bool less = at < lo + len && skey[at] + RISE * (unsigned)at < v;
+    const int c = __popcll(__ballot(less));      // (ascending: the first c lanes)
     if (c == 0) return lo;
     const int64_t from = lo + (int64_t)(c - 1) * step + 1;
     const int64_t to = c < 64 && lo + (int64_t)c * step < lo + len ? lo + (int64_t)c * step : lo + len;
@@ -250,46 +323,109 @@ __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_
   return lo;
 }
 
-// one wave per row of the table and 64 * N columns
+// The rows of the table, each followed by its sorted positions, are one sequence of vocab + n entries: row v is entry
+// v + (positions of smaller keys).  It is cut into stretches of `stretch` entries, and a wave owns the rows that lie in its
+// stretch (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows
+// without a position as zeros.  So no wave has much more to do than another, whatever the tokens are.  It walks 64 sorted
+// positions at a time; the dy rows of several tokens are on their way together.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
-  const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v >= (int64_t)a.vocab) return;
+  const unsigned id = wave_id(), unit = id / a.slices;
   const int lane = threadIdx.x & 63;
-  const int64_t b = wave_lower_bound(a.skey, a.n, (unsigned)v, lane);
-  const int64_t e = b + wave_lower_bound(a.skey + b, a.n - b, (unsigned)v + 1, lane);
-  const int col = (blockIdx.y * 64 + lane) * N;
-  if (col >= a.width) return;
-  const int left = a.width - col;
+  const int64_t d0 = (int64_t)unit * a.stretch, d1 = d0 + a.stretch;
+  if (d0 >= (int64_t)a.vocab + a.n) return;
+  const int col = ((int)(id - unit * a.slices) * 64 + lane) * N;
+  const Columns<T, N> c = {col, a.width - col};
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+  T* dw = reinterpret_cast<T*>(a.dw);
   float s[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) s[k] = 0.f;
-  const int64_t g1 = (b + GROUP - 1) / GROUP, g2 = e / GROUP;               // whole groups [g1, g2)
-  if (e > b) {
-    if (g1 >= g2) {
-      add_rows<T, N>(a, b, e, col, s);
-    } else {
-      add_rows<T, N>(a, b, g1 * GROUP, col, s);
-      const int64_t h1 = (g1 + GROUP - 1) / GROUP, h2 = g2 / GROUP;         // whole groups of groups
-      const int64_t c1 = h1 < h2 ? h1 * GROUP : g2, c2 = h1 < h2 ? h2 * GROUP : g2;
-      for (int64_t c = g1; c < c1; ++c) add_row<float, N>(a.part1 + c * a.width + col, left, s);
-      for (int64_t c = h1; c < h2; ++c) add_row<float, N>(a.part2 + c * a.width + col, left, s);
-      for (int64_t c = c2; c < g2; ++c) add_row<float, N>(a.part1 + c * a.width + col, left, s);
-      add_rows<T, N>(a, g2 * GROUP, e, col, s);
-    }
-    if (a.act) {
-      float w[N];
-      const T* t = reinterpret_cast<const T*>(a.table) + v * a.ldt + col;
-      if (left >= N) gvd_load<T, N>(t, w); else gvd_load_part<T, N>(t, left, w);
-#pragma unroll
-      for (int k = 0; k < N; ++k) s[k] = w[k] * a.scale > 0.f ? s[k] * a.scale : 0.f;
-    } else {
-#pragma unroll
-      for (int k = 0; k < N; ++k) s[k] *= a.scale;
-    }
+  // the first row of the stretch, `cur`, and its first position, `i`: behind i positions and d0 - i rows, or, if row d0 - i began
+  // before the stretch, behind the rest of its positions
+  int64_t i = wave_lower_bound<1>(a.skey, 0, a.n, (unsigned)d0, lane);
+  unsigned cur = (unsigned)(d0 - i);
+  if (i > 0 && i < a.n && a.skey[i - 1] == cur) {
+    const unsigned long long same = __ballot(i + lane < a.n && a.skey[i + lane] == cur);
+    i = ~same ? i + __popcll(same) : wave_lower_bound<0>(a.skey, i + 64, a.n, cur + 1, lane);
+    ++cur;
+  } else if (i > 0 && i == a.n && a.skey[i - 1] == cur) {
+    ++cur;
   }
-  T* o = reinterpret_cast<T*>(a.dw) + v * (int64_t)a.width + col;
-  if (left >= N) gvd_store<T, N>(o, s); else gvd_store_part<T, N>(o, left, s);
+  const auto zeros = [&](int64_t to) {           // rows cur ... to - 1 have no positions
+    float x[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = 0.f;
+    for (; (int64_t)cur < to; ++cur)
+      if (c.left > 0) c.store(dw + (int64_t)cur * a.width, x);
+  };
+  const auto finish = [&](unsigned v) {          // row v is s
+    if (c.left > 0) {
+      float x[N];
+      if (a.act) {
+        const typename Columns<T, N>::Raw w = c.fetch(reinterpret_cast<const T*>(a.table) + (int64_t)v * a.ldt);
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = (float)w[k] * a.scale > 0.f ? s[k] * a.scale : 0.f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = s[k] * a.scale;
+      }
+      c.store(dw + (int64_t)v * a.width, x);
+    }
+    cur = v + 1;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = 0.f;
+  };
+  while (true) {
+    const unsigned key = i + lane < a.n ? a.skey[i + lane] : a.vocab;
+    const unsigned which = i + lane < a.n ? a.spos[i + lane] : 0;
+    const unsigned first = __builtin_amdgcn_readfirstlane(key), last = __builtin_amdgcn_readlane(key, 63);
+    zeros((int64_t)first < d1 - i ? (int64_t)first : d1 - i);
+    if (first >= a.vocab || (int64_t)first >= d1 - i) break;
+    if (first == last) {                         // 64 positions or more of one token
+      const int64_t e = wave_lower_bound<0>(a.skey, i + 64, a.n, first + 1, lane);
+      const int64_t g1 = (i + GROUP - 1) / GROUP, g2 = e / GROUP;                 // whole groups (there is one at least)
+      const Columns<float, N> cf = {c.col, c.left};
+      add_positions<T, N>(a, i, g1 * GROUP, lane, c, s);
+      const int64_t h1 = (g1 + GROUP - 1) / GROUP, h2 = g2 / GROUP;               // whole groups of groups
+      if (a.n < LEVEL2_FROM || h1 >= h2) {
+        add_partials<N>(a.part1, a.width, g1, g2, lane, cf, s);
+      } else {
+        add_partials<N>(a.part1, a.width, g1, h1 * GROUP, lane, cf, s);
+        add_partials<N>(a.part2, a.width, h1, h2, lane, cf, s);
+        add_partials<N>(a.part1, a.width, h2 * GROUP, g2, lane, cf, s);
+      }
+      add_positions<T, N>(a, g2 * GROUP, e, lane, c, s);
+      finish(first);
+      i = e;
+      continue;
+    }
+    // the tokens that end within these 64 positions, up to the first one whose row lies behind the stretch
+    const unsigned left = __shfl_up(key, 1, GVD_WAVE);
+    const unsigned long long behind = __ballot((lane == 0 || key != left) && (key >= a.vocab || (int64_t)key + i + lane >= d1));
+    int count = __popcll(__ballot(key != last));
+    if (behind) count = count < __ffsll(behind) - 1 ? count : __ffsll(behind) - 1;
+    constexpr int BATCH = 8;
+    for (int j0 = 0; j0 < count; j0 += BATCH) {
+      typename Columns<T, N>::Raw x[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (j0 + k < count) x[k] = c.fetch(dy + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, j0 + k) * a.ld);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        if (j0 + k < count) {
+          const unsigned v = __builtin_amdgcn_readlane(key, j0 + k);
+#pragma unroll
+          for (int e = 0; e < N; ++e) s[e] += (float)x[k][e];
+          if (__builtin_amdgcn_readlane(key, j0 + k + 1) != v) {                  // (count <= 63: lane 63 belongs to a later token)
+            zeros(v);
+            finish(v);
+          }
+        }
+      }
+    }
+    i += count;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -300,6 +436,8 @@ int lane_columns(int width, int dtype) {
   while (n < most && 64 * n < width) n *= 2;
   return n;
 }
+
+constexpr int64_t MAX_WAVES = (1ll << 26) - 4;      // (a launch holds fewer than 2^32 threads)
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -343,25 +481,33 @@ bool bad_shape(int64_t n, int64_t vocab, int width, int dtype) {
 template <typename T, int N>
 int launch_fwd(const void* tok, int tok64, int64_t n, const void* table, int64_t ld, int64_t vocab, int width, float scale,
                int act, void* out, int64_t ldo, hipStream_t st) {
-  const dim3 grid((unsigned)((n + 3) / 4), (unsigned)((width + 64 * N - 1) / (64 * N)));
-  hipLaunchKernelGGL((embedding_fwd_kernel<T, N>), grid, dim3(256), 0, st, tok, tok64, n, reinterpret_cast<const T*>(table), ld,
-                     (unsigned)vocab, width, scale, act, reinterpret_cast<T*>(out), ldo);
+  const unsigned slices = (unsigned)((width + 64 * N - 1) / (64 * N));
+  const bool many = n * slices >= 16384;   // (four rows a wave still leave four waves to every SIMD)
+  const int64_t waves = (many ? (n + 3) / 4 : n) * slices;
+  if (waves > MAX_WAVES) return GVD_EINVAL;
+  hipLaunchKernelGGL((many ? embedding_fwd_kernel<T, N, 4> : embedding_fwd_kernel<T, N, 1>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
+                     st, tok, tok64, n, reinterpret_cast<const T*>(table), ld, (unsigned)vocab, width, scale, act,
+                     reinterpret_cast<T*>(out), ldo, slices);
   GVD_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T, int N> int launch_sums(const SumArgs& a, hipStream_t st) {
-  const unsigned slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
-  const int64_t g1 = a.n / GROUP, g2 = a.n / (GROUP * GROUP);
-  if (g1) {
-    hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4), slices), dim3(256), 0, st, a);
+template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
+  a.slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
+  const int64_t g1 = a.n / GROUP * a.slices, g2 = a.n / (GROUP * GROUP) * a.slices;
+  a.stretch = 8;                           // entries a wave, up to 64, that still leave four waves to every SIMD
+  while (a.stretch < 64 && ((int64_t)a.vocab + a.n) / a.stretch * a.slices >= 2 * 4096) a.stretch *= 2;
+  const int64_t owners = ((int64_t)a.vocab + a.n + a.stretch - 1) / a.stretch * a.slices;
+  if (g1 > MAX_WAVES || owners > MAX_WAVES) return GVD_EINVAL;
+  if (a.n >= 64) {
+    hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
     GVD_CHECK_LAUNCH();
   }
-  if (g2) {
-    hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4), slices), dim3(256), 0, st, a);
+  if (a.n >= LEVEL2_FROM) {
+    hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
     GVD_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL((token_rows_kernel<T, N>), dim3((unsigned)((a.vocab + 3) / 4), slices), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((token_rows_kernel<T, N>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
   GVD_CHECK_LAUNCH();
   return 0;
 }

@@ -17,14 +17,18 @@ namespace {
 constexpr int CHUNK = GVD_GRAD_CHUNK;
 constexpr int MAX_GRID = 1024;
 
-__device__ __forceinline__ int tensor_of_chunk(const gvd_grad_group& g, unsigned chunk) {
-  int lo = 0, hi = g.count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (g.chunk0[mid] <= chunk) lo = mid; else hi = mid;
+// A chunk's tensor: the lanes hold the tensors' first chunks (two each) and count those at or before it.
+struct FirstChunks {
+  unsigned a, b;
+  __device__ __forceinline__ FirstChunks(const gvd_grad_group& g) {
+    const int lane = threadIdx.x & 63;
+    a = lane < g.count ? g.chunk0[lane] : 0xffffffffu;
+    b = lane + 64 < g.count ? g.chunk0[lane + 64] : 0xffffffffu;
   }
-  return lo;
-}
+  __device__ __forceinline__ int tensor_of(unsigned chunk) const {
+    return __popcll(__ballot(a <= chunk)) + __popcll(__ballot(b <= chunk)) - 1;
+  }
+};
 
 __device__ __forceinline__ double block_sum_f64(double v, double* s_red) {
 #pragma unroll
@@ -34,9 +38,21 @@ __device__ __forceinline__ double block_sum_f64(double v, double* s_red) {
   return (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
 }
 
+// A full chunk is loaded as a whole, 16 bytes a lane and instruction, before its first element is used.
 template <typename T> __device__ __forceinline__ double chunk_sumsq(const T* p, int64_t n) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), VECS = CHUNK / (256 * N);
+  typedef typename GvdVec<T, N>::loose Loose;
   double s = 0.0;
+  if (n == CHUNK) {
+    typename GvdVec<T, N>::type x[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) x[i] = *reinterpret_cast<const Loose*>(p + (i * 256 + threadIdx.x) * N);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) { const double v = (float)x[i][k]; s = fma(v, v, s); }
+    return s;
+  }
   const int64_t nv = n / N * N;
   for (int64_t i = (int64_t)threadIdx.x * N; i < nv; i += 256 * N) {
     float v[N];
@@ -51,9 +67,10 @@ template <typename T> __device__ __forceinline__ double chunk_sumsq(const T* p, 
 __global__ __launch_bounds__(256) void grad_sumsq_kernel(const gvd_grad_group g, double* __restrict__ partials) {
   __shared__ double s_red[4];
   double s = 0.0;
+  const FirstChunks first(g);
   const unsigned chunks = g.chunk0[g.count];
   for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int t = tensor_of_chunk(g, c);
+    const int t = first.tensor_of(c);
     const int64_t e0 = (int64_t)(c - g.chunk0[t]) * CHUNK;
     const int64_t n = g.n[t] - e0 < CHUNK ? g.n[t] - e0 : CHUNK;
     if (g.src_type[t] == GVD_F32) s += chunk_sumsq(reinterpret_cast<const float*>(g.src[t]) + e0, n);
@@ -68,7 +85,21 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(const gvd_grad_group g,
 struct Factor { float f, p; };
 
 template <typename TI, typename TO> __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, Factor f) {
-  constexpr int N = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
+  constexpr int N = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO)), VECS = CHUNK / (256 * N);
+  if (n == CHUNK) {
+    typename GvdVec<TI, N>::type x[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+      x[i] = *reinterpret_cast<const typename GvdVec<TI, N>::loose*>(src + (i * 256 + threadIdx.x) * N);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      float v[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = (float)x[i][k] * f.f * f.p;
+      gvd_store<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
+    }
+    return;
+  }
   const int64_t nv = n / N * N;
   for (int64_t i = (int64_t)threadIdx.x * N; i < nv; i += 256 * N) {
     float v[N];
@@ -98,8 +129,11 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const gvd_grad_group g,
   const bool tiny = factor < 0x1p-100;
   const Factor f = {(float)(tiny ? factor * 0x1p100 : factor), tiny ? 0x1p-100f : 1.0f};
   const unsigned chunks = g.count ? g.chunk0[g.count] : 0;
-  for (unsigned k = blockIdx.x; k < chunks; k += gridDim.x) {
-    const int t = tensor_of_chunk(g, k);
+  const FirstChunks first(g);
+  // from the last chunk to the first: what gvd_grad_sumsq read last is still in the 256 MB cache
+  for (unsigned at = blockIdx.x; at < chunks; at += gridDim.x) {
+    const unsigned k = chunks - 1 - at;
+    const int t = first.tensor_of(k);
     if (factor == 1.0 && g.src[t] == g.dst[t]) continue;                       // in place and nothing to clip
     const int64_t e0 = (int64_t)(k - g.chunk0[t]) * CHUNK;
     const int64_t n = g.n[t] - e0 < CHUNK ? g.n[t] - e0 : CHUNK;

@@ -342,9 +342,16 @@ def stream_ptr():
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def stream_on(device):
-    """The current stream of `device` (which need not be the current device)."""
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def run_on(device, fn, what, *args):
+    """fn(*args, the current stream of `device`) with `device` current, whichever device is current for the caller."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc, what)
 
 
 def ptr(t):

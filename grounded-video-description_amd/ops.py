@@ -8,7 +8,7 @@ import os
 import torch
 
 from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs, DxGroup, GemmArgs, GemmSeg, GreedyArgs,
-                  GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr, require_cuda_f32, stream_on, stream_ptr)
+                  GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr, require_cuda_f32, run_on, stream_ptr)
 
 # ---------------------------------------------------------------------------------------------------------------------
 # "No library GEMM on the hot path" as an invariant.  Every place where a product or softmax of the path would leave
@@ -1887,10 +1887,8 @@ def _embedding_fwd(tokens, weight, scale, act):
     n = tokens.numel()
     out = torch.empty(tokens.shape + (E,), dtype=weight.dtype, device=weight.device)
     if n and E:
-        with torch.cuda.device(weight.device):
-            check(lib().gvd_embedding_fwd(ptr(tokens), tokens.dtype == torch.int64, n, ptr(weight), weight.stride(0) if V > 1 else E, V,
-                                          E, DTYPES[weight.dtype], scale, act, ptr(out), E, stream_on(weight.device)),
-                  'gvd_embedding_fwd')
+        run_on(weight.device, lib().gvd_embedding_fwd, 'gvd_embedding_fwd', tokens.data_ptr(), tokens.dtype == torch.int64, n,
+               weight.data_ptr(), weight.stride(0) if V > 1 else E, V, E, DTYPES[weight.dtype], scale, act, out.data_ptr(), E)
     return out
 
 
@@ -1913,12 +1911,12 @@ class _EmbeddingFn(torch.autograd.Function):
         if E > 1 and dy2.stride(1) != 1:       # (a gradient broadcast over the rows, stride 0, is read in place)
             dy2 = dy2.contiguous()
         dw = torch.empty(V, E, dtype=dtype, device=dev)
-        need = lib().gvd_embedding_bwd_workspace_bytes(n, V, E)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            check(lib().gvd_embedding_bwd(ptr(tokens), tokens.dtype == torch.int64, n, ptr(dy2), dy2.stride(0), ptr(weight),
-                                          (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype], scale, act, pad, ptr(dw), ptr(ws),
-                                          ws.numel(), stream_on(dev)), 'gvd_embedding_bwd')
+        l = lib()
+        need = l.gvd_embedding_bwd_workspace_bytes(n, V, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        run_on(dev, l.gvd_embedding_bwd, 'gvd_embedding_bwd', tokens.data_ptr(), tokens.dtype == torch.int64, n, dy2.data_ptr(),
+               dy2.stride(0), weight.data_ptr() if act else None, (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype],
+               scale, act, pad, dw.data_ptr(), ws.data_ptr(), need)
         return None, dw, None, None, None
 
 
@@ -1980,47 +1978,55 @@ def beam_select(logits, scores, width=None, finished=None, eos=None):
         logits = logits.contiguous()
     scores = scores.contiguous()
     a = BeamSelectArgs()
-    a.logits, a.ld, a.dtype = ptr(logits), max(logits.stride(0), V), DTYPES[logits.dtype]
+    a.logits, a.ld, a.dtype = logits.data_ptr(), max(logits.stride(0), V), DTYPES[logits.dtype]
     a.B, a.K, a.V, a.W, a.eos = B, K, V, W, -1 if eos is None else eos
-    a.scores = ptr(scores)
+    a.scores = scores.data_ptr()
     if finished is not None:
         finished = finished.contiguous()
-        a.finished = ptr(finished)
+        a.finished = finished.data_ptr()
     out = torch.empty(B, W, dtype=torch.float32, device=dev)
-    ids = torch.empty(2, B, W, dtype=torch.int64, device=dev)
-    parent, word = ids.unbind(0)
+    parent = torch.empty(B, W, dtype=torch.int64, device=dev)
+    word = torch.empty(B, W, dtype=torch.int64, device=dev)
     done = None
     if eos is not None:
         done = torch.empty(B, W, dtype=torch.uint8 if finished is None else finished.dtype, device=dev)
-        a.out_finished = ptr(done)
-    need = lib().gvd_beam_select_workspace_bytes(B, K, V, W)
+        a.out_finished = done.data_ptr()
+    l = lib()
+    need = l.gvd_beam_select_workspace_bytes(B, K, V, W)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    a.out_scores, a.parent, a.word = ptr(out), ptr(parent), ptr(word)
-    a.workspace, a.workspace_bytes = ptr(ws), need
-    with torch.cuda.device(dev):
-        check(lib().gvd_beam_select(C.byref(a), stream_on(dev)), 'gvd_beam_select')
+    a.out_scores, a.parent, a.word = out.data_ptr(), parent.data_ptr(), word.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    run_on(dev, l.gvd_beam_select, 'gvd_beam_select', C.byref(a))
     return out, parent, word, done
 
 
 def _rows_view(x, dim):
     """(outer, outer stride, row stride, row bytes) in bytes of x seen as [outer, rows = x.shape[dim], row]; None where its
     strides do not allow that view."""
-    size = x.element_size()
+    shape, strides, size = x.shape, x.stride(), x.element_size()
     inner = 1
-    for d in range(x.dim() - 1, dim, -1):
-        if x.shape[d] != 1 and x.stride(d) != inner:
+    if x.is_contiguous():
+        for d in range(dim + 1, len(shape)):
+            inner *= shape[d]
+        row = inner * size
+        outer = 1
+        for d in range(dim):
+            outer *= shape[d]
+        return outer, shape[dim] * row, row, row
+    for d in range(len(shape) - 1, dim, -1):
+        if shape[d] != 1 and strides[d] != inner:
             return None
-        inner *= x.shape[d]
+        inner *= shape[d]
     outer, ostride = 1, 0
     for d in range(dim - 1, -1, -1):
-        if x.shape[d] == 1:
+        if shape[d] == 1:
             continue
         if outer == 1:
-            ostride = x.stride(d)
-        elif x.stride(d) != ostride * outer:
+            ostride = strides[d]
+        elif strides[d] != ostride * outer:
             return None
-        outer *= x.shape[d]
-    return outer, ostride * size, x.stride(dim) * size, inner * size
+        outer *= shape[d]
+    return outer, ostride * size, strides[dim] * size, inner * size
 
 
 def _extent(x):
@@ -2077,13 +2083,17 @@ def reorder_rows(states, parent, dim=0, out=None):
         if src is None:
             x = x.contiguous()
             src = _rows_view(x, d)
-        dst = _rows_view(y, d)
-        ok, need = dst is not None, 0 if dst is None else dst[3]
-        for stride, count in sorted([(dst[1], dst[0]), (dst[2], n)]) if ok else []:
-            if count > 1:
-                ok, need = ok and stride >= need, stride * (count - 1) + need
-        if not ok:
-            raise GvdHipError('reorder_rows: result %d is not made of whole rows of their own (strides %s)' % (i, y.stride()))
+        if out is None:
+            row = src[3]
+            dst = (src[0], n * row, row, row)
+        else:
+            dst = _rows_view(y, d)
+            ok, need = dst is not None, 0 if dst is None else dst[3]
+            for stride, count in sorted([(dst[1], dst[0]), (dst[2], n)]) if ok else []:
+                if count > 1:
+                    ok, need = ok and stride >= need, stride * (count - 1) + need
+            if not ok:
+                raise GvdHipError('reorder_rows: result %d is not made of whole rows of their own (strides %s)' % (i, y.stride()))
         items.append((x, y, src, dst))
     if not parent.is_cuda:
         raise GvdHipError('reorder_rows: non-GPU tensor; there is no CPU fallback')
@@ -2095,14 +2105,12 @@ def reorder_rows(states, parent, dim=0, out=None):
                 raise GvdHipError('reorder_rows: a result overlaps a state or another result')
             end = max(end, b)
             wend = max(wend, b) if written else wend
-    with torch.cuda.device(dev):
-        for k in range(0, len(items), REORDER_MAX_TENSORS):
-            part = items[k:k + REORDER_MAX_TENSORS]
-            g = ReorderGroup()
-            g.count = len(part)
-            for i, (x, y, (outer, so, sr, row), (_, do, dr, _)) in enumerate(part):
-                t = g.t[i]
-                t.src, t.dst = x.data_ptr(), y.data_ptr()
-                t.outer, t.src_outer, t.dst_outer, t.src_row, t.dst_row, t.row_bytes = outer, so, do, sr, dr, row
-            check(lib().gvd_reorder_rows(C.byref(g), ptr(parent), rows, n, stream_on(dev)), 'gvd_reorder_rows')
+    for k in range(0, len(items), REORDER_MAX_TENSORS):
+        part = items[k:k + REORDER_MAX_TENSORS]
+        g = ReorderGroup()
+        g.count = len(part)
+        for t, (x, y, (outer, so, sr, row), (_, do, dr, _)) in zip(g.t, part):
+            t.src, t.dst, t.outer = x.data_ptr(), y.data_ptr(), outer
+            t.src_outer, t.dst_outer, t.src_row, t.dst_row, t.row_bytes = so, do, sr, dr, row
+        run_on(dev, lib().gvd_reorder_rows, 'gvd_reorder_rows', C.byref(g), parent.data_ptr(), rows, n)
     return results

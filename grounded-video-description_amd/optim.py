@@ -9,11 +9,13 @@ never written back (so, unlike after clip_grad_norm_, `.grad` still holds the UN
 """
 import ctypes as C
 import math
+import operator
 
+import numpy as np
 import torch
 
 from .hip import (DTYPES, GRAD_CHUNK, GRAD_MAX_TENSORS, OPT_CHUNK, OPT_MAX_TENSORS, GradClip, GradGroup, GvdHipError, OptGroup, check,
-                  lib, ptr, stream_on, stream_ptr)
+                  lib, ptr, run_on, stream_ptr)
 
 
 class ClipAdam(torch.optim.Adam):
@@ -144,8 +146,15 @@ class ClipAdam(torch.optim.Adam):
 
 # ---------------------------------------------------------------------------------------------------------------------
 # The global gradient norm and clipping as operators of their own (csrc/grad_clip.hip), for optimisers other than ClipAdam:
-# fp32, bf16 and fp16 gradients, mixed, clipped in place or written - unscaled - into master gradients of another type.
+# fp32, bf16 and fp16 gradients, mixed, clipped in place or written - unscaled - into master gradients of another type.  What
+# is looked at per tensor goes through map() and numpy: with hundreds of small gradients the host is what a call waits for.
 # ---------------------------------------------------------------------------------------------------------------------
+_DTYPE = operator.attrgetter('dtype')
+_T = torch.Tensor
+_GROUP_FIELDS = {f: (getattr(GradGroup, f).offset, t) for f, t in (('src', np.int64), ('dst', np.int64), ('n', np.int64),
+                                                                   ('chunk0', np.uint32), ('src_type', np.uint8), ('dst_type', np.uint8))}
+
+
 def _dense(t):
     """t's elements fill one stretch of memory, each at a place of its own (in whatever order)."""
     if t.is_contiguous():
@@ -158,78 +167,113 @@ def _dense(t):
     return True
 
 
+def _repeats(t):
+    """Several elements of t share a place."""
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
+
+
 def _check_grads(grads, what):
-    """The gradients that have elements; dense float tensors on one GPU."""
+    """Dense float tensors on one GPU."""
+    for i, g in enumerate(grads) if not DTYPES.keys() >= set(map(_DTYPE, grads)) else ():
+        if g.dtype not in DTYPES:
+            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s' % (what, i, g.dtype))
     for i, g in enumerate(grads):
-        if g.dtype not in DTYPES or g.layout != torch.strided:
-            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s %s'
-                              % (what, i, g.layout, g.dtype))
-        if g.device != grads[0].device:
-            raise GvdHipError('%s: gradients on %s and %s' % (what, grads[0].device, g.device))
-    if grads and not grads[0].is_cuda:
+        if g.layout != torch.strided:
+            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s' % (what, i, g.layout))
+    devices = set(map(_T.get_device, grads))
+    if len(devices) > 1:
+        raise GvdHipError('%s: gradients on several devices (%s)' % (what, sorted(devices)))
+    if devices and not grads[0].is_cuda:
         raise GvdHipError('%s: the gradients are not on the GPU; there is no CPU fallback' % what)
-    return [g for g in grads if g.numel()]
 
 
-def _no_overlap(tensors, what):
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
+class _Tensors:
+    """Addresses, sizes and type codes of a list of tensors."""
+
+    def __init__(self, tensors, like=None):
+        self.ptr = np.array(list(map(_T.data_ptr, tensors)), np.int64)
+        self.n = like.n if like is not None else np.array(list(map(_T.numel, tensors)), np.int64)
+        first = tensors[0].dtype
+        types = list(map(_DTYPE, tensors))
+        if types.count(first) == len(types):
+            self.code = np.full(len(types), DTYPES[first], np.uint8)
+        else:
+            self.code = np.array([DTYPES[t] for t in types], np.uint8)
+        self.end = self.ptr + self.n * np.where(self.code == 0, 4, 2)
+
+
+def _any_overlap(starts, ends):
+    order = np.argsort(starts)
+    return len(order) > 1 and bool((np.maximum.accumulate(ends[order])[:-1] > starts[order][1:]).any())
+
+
+def _check_written(src, dst, what):
+    """No two written tensors share memory; a result is its own gradient or shares memory with none."""
+    if src is dst:
+        if _any_overlap(dst.ptr, dst.end):
             raise GvdHipError('%s: two of the tensors to be written share memory' % what)
+        return
+    other = ~((src.ptr == dst.ptr) & (src.code == dst.code))
+    if not _any_overlap(np.concatenate([dst.ptr, src.ptr[other]]), np.concatenate([dst.end, src.end[other]])):
+        return
+    if _any_overlap(dst.ptr, dst.end):
+        raise GvdHipError('%s: two of the tensors to be written share memory' % what)
+    # (gradients may overlap each other, results nothing: look at each gradient's neighbours among the results)
+    order = np.argsort(dst.ptr)
+    starts, ends = dst.ptr[order], dst.end[order]
+    k = np.searchsorted(ends, src.ptr[other], side='right')          # the first result that ends behind the gradient's start
+    hit = (k < len(starts)) & (starts[np.minimum(k, len(starts) - 1)] < src.end[other])
+    if bool(hit.any()):
+        raise GvdHipError('%s: a result shares memory with a gradient that is not its own' % what)
 
 
-def _grad_groups(grads, out):
-    """Launch arguments of at most GRAD_MAX_TENSORS tensors each; out: the tensors to be written (None: the norm alone)."""
+def _grad_groups(src, dst):
+    """Launch arguments of at most GRAD_MAX_TENSORS tensors each; dst None: the norm alone."""
     groups = []
-    for k in range(0, len(grads), GRAD_MAX_TENSORS):
-        part = grads[k:k + GRAD_MAX_TENSORS]
+    chunks = -(-src.n // GRAD_CHUNK)
+    for k in range(0, len(src.n), GRAD_MAX_TENSORS):
+        part = slice(k, k + GRAD_MAX_TENSORS)
         g = GradGroup()
-        g.count = len(part)
-        ns = [t.numel() for t in part]
-        g.src[:len(part)] = [t.data_ptr() for t in part]
-        g.n[:len(part)] = ns
-        g.src_type[:len(part)] = [DTYPES[t.dtype] for t in part]
-        at, firsts = 0, [0]
-        for n in ns:
-            at += -(-n // GRAD_CHUNK)
-            firsts.append(at)
-        g.chunk0[:len(part) + 1] = firsts
-        if out is not None:
-            w = out[k:k + GRAD_MAX_TENSORS]
-            g.dst[:len(part)] = [t.data_ptr() for t in w]
-            g.dst_type[:len(part)] = [DTYPES[t.dtype] for t in w]
+        count = g.count = len(src.n[part])
+
+        def put(field, values, at=0):
+            offset, dtype = _GROUP_FIELDS[field]
+            np.frombuffer(g, dtype, count + at, offset)[at:] = values
+        put('src', src.ptr[part])
+        put('n', src.n[part])
+        put('src_type', src.code[part])
+        put('chunk0', np.cumsum(chunks[part]), 1)
+        if dst is not None:
+            put('dst', dst.ptr[part])
+            put('dst_type', dst.code[part])
         groups.append(g)
     return groups
 
 
-def _norm_and_scale(grads, out, max_norm, inv_scale, error_if_nonfinite, what):
-    """grads: live, dense.  The norm (device scalar); out (tensors like grads) = the clipped gradients, None = the norm alone."""
-    dev = grads[0].device
+def _norm_and_scale(dev, src, dst, max_norm, inv_scale, error_if_nonfinite, what):
+    """The norm of src (device scalar); dst = the clipped gradients, None = the norm alone."""
+    if int(src.n.max()) > GRAD_CHUNK * 0x7fffffff // len(src.n):
+        raise GvdHipError('%s: the gradients are too large for one call' % what)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    groups = _grad_groups(grads, out)
+    groups = _grad_groups(src, dst)
     l = lib()
-    parts = []
-    for g in groups:
-        n = l.gvd_grad_parts(C.byref(g))
-        if n <= 0:
-            raise GvdHipError('%s: the gradients are too large for one call' % what)
-        parts.append(n)
-    partials = torch.empty(sum(parts), dtype=torch.float64, device=dev)
+    parts = [l.gvd_grad_parts(C.byref(g)) for g in groups]
+    if min(parts) <= 0:
+        raise GvdHipError('%s: gvd_grad_parts refused the gradients' % what)
+    total = sum(parts)
+    partials = torch.empty(total, dtype=torch.float64, device=dev)
     c = GradClip(max_norm, inv_scale)
-    with torch.cuda.device(dev):
-        st = stream_on(dev)
-        at = partials.data_ptr()
-        for g, n in zip(groups, parts):
-            check(l.gvd_grad_sumsq(C.byref(g), at, st), 'gvd_grad_sumsq')
-            at += 8 * n
-        if out is None or error_if_nonfinite:
-            check(l.gvd_grad_scale(C.byref(GradGroup()), C.byref(c), ptr(partials), sum(parts), ptr(norm), st), 'gvd_grad_scale')
-            if error_if_nonfinite and not bool(torch.isfinite(norm)):
-                raise RuntimeError('%s: the total norm of the gradients is not finite (%s); they were not clipped' % (what, float(norm)))
-        if out is not None:
-            for i, g in enumerate(groups):
-                check(l.gvd_grad_scale(C.byref(g), C.byref(c), ptr(partials), sum(parts), None if i else ptr(norm), st),
-                      'gvd_grad_scale')
+    at = first = partials.data_ptr()
+    for g, n in zip(groups, parts):
+        run_on(dev, l.gvd_grad_sumsq, 'gvd_grad_sumsq', C.byref(g), at)
+        at += 8 * n
+    if dst is None or error_if_nonfinite:
+        run_on(dev, l.gvd_grad_scale, 'gvd_grad_scale', C.byref(GradGroup()), C.byref(c), first, total, norm.data_ptr())
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
+            raise RuntimeError('%s: the total norm of the gradients is not finite (%s); they were not clipped' % (what, float(norm)))
+    if dst is not None:
+        for i, g in enumerate(reversed(groups)):       # (backwards: what was read last is still in the cache)
+            run_on(dev, l.gvd_grad_scale, 'gvd_grad_scale', C.byref(g), C.byref(c), first, total, None if i else norm.data_ptr())
     return norm
 
 
@@ -242,6 +286,10 @@ def _check_clip(max_norm, inv_scale, what):
     return max_norm, inv_scale
 
 
+def _no_gradients(grads):
+    return torch.zeros((), device=grads[0].device if grads else 'cuda')
+
+
 @torch.no_grad()
 def grad_norm(grads, inv_scale=1.0):
     """inv_scale * the L2 norm of all elements of all tensors, a float32 scalar on their device (0 for none).  Summed in fp64 in a
@@ -249,10 +297,11 @@ def grad_norm(grads, inv_scale=1.0):
     what = 'grad_norm'
     _, inv_scale = _check_clip(0.0, inv_scale, what)
     grads = list(grads)
-    live = _check_grads(grads, what)
+    _check_grads(grads, what)
+    live = [g if _dense(g) else g.contiguous() for g in grads if g.numel()]
     if not live:
-        return torch.zeros((), device=grads[0].device if grads else 'cuda')
-    return _norm_and_scale([g if _dense(g) else g.contiguous() for g in live], None, 0.0, inv_scale, False, what)
+        return _no_gradients(grads)
+    return _norm_and_scale(live[0].device, _Tensors(live), None, 0.0, inv_scale, False, what)
 
 
 @torch.no_grad()
@@ -272,53 +321,49 @@ def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=Fals
         if len(out) != len(grads):
             raise GvdHipError('%s: %d gradients, %d results' % (what, len(grads), len(out)))
         for i, (g, o) in enumerate(zip(grads, out)):
-            if o.device != g.device or o.dtype not in DTYPES or o.shape != g.shape:
+            if o.dtype not in DTYPES or o.shape != g.shape or o.get_device() != g.get_device():
                 raise GvdHipError('%s: result %d must be a float32 / bfloat16 / float16 tensor %s on %s' % (what, i, tuple(g.shape),
                                                                                                             g.device))
-        out = [o for o in out if o.numel()]
-    live = _check_grads(grads, what)
-    if not live:
-        return torch.zeros((), device=grads[0].device if grads else 'cuda')
-    if out is None:
-        src = [g if _dense(g) else g.contiguous() for g in live]
-        dst, back = src, [(g, s) for g, s in zip(live, src) if s is not g]
-        for g, _ in back:
-            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-                raise GvdHipError('%s: a gradient of strides %s cannot be clipped in place' % (what, g.stride()))
-    else:
+    _check_grads(grads, what)
+    written = grads if out is None else out
+    if not all(map(_T.numel, grads)):
+        keep = [i for i, g in enumerate(grads) if g.numel()]
+        grads, written = [grads[i] for i in keep], [written[i] for i in keep]
+    if not grads:
+        return _no_gradients(written)
+    src, dst, back = grads, written, []
+    if not (all(map(_T.is_contiguous, grads)) and (out is None or all(map(_T.is_contiguous, written)))):
         # element i of a result belongs to element i of its gradient: same order in memory, or both in row-major order
-        src, dst, back = [], [], []
-        for g, o in zip(live, out):
-            if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-                raise GvdHipError('%s: a result of strides %s cannot be written' % (what, o.stride()))
+        src, dst = [], []
+        for g, o in zip(grads, written):
+            if _repeats(o):
+                raise GvdHipError('%s: a tensor of strides %s cannot be written' % (what, o.stride()))
             same = g.stride() == o.stride() and _dense(g)
             src.append(g if same else g.contiguous())
-            dst.append(o if same or o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format))
+            dst.append(o if same or o.is_contiguous() else src[-1] if o is g else torch.empty_like(o, memory_format=torch.contiguous_format))
             if dst[-1] is not o:
                 back.append((o, dst[-1]))
-    _no_overlap(dst, what)
-    if out is not None:
-        _no_partial_alias(src, dst, what)
-    norm = _norm_and_scale(src, dst, max_norm, inv_scale, error_if_nonfinite, what)
-    for o, d in back:
-        o.copy_(d)
-    written = live if out is None else out
-    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    s = _Tensors(src)
+    d = s if src is dst or all(map(operator.is_, src, dst)) else _Tensors(dst, s)
+    _check_written(s, d, what)
+    for o, _ in back:
+        _check_scattered(o, src, dst, what)
+    norm = _norm_and_scale(grads[0].device, s, d, max_norm, inv_scale, error_if_nonfinite, what)
+    for o, x in back:
+        o.copy_(x)
+    try:
+        torch.autograd.graph.increment_version(written)
+    except RuntimeError:                                 # (inference tensors have no version)
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
 
 
-def _no_partial_alias(src, dst, what):
-    """A result is its own gradient (clipped in place) or shares no memory with any gradient."""
-    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, 0) for i, t in enumerate(src)] +
-                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, 1) for i, t in enumerate(dst)])
-    open_ = []
-    for a, b, i, written in spans:
-        open_ = [s for s in open_ if s[1] > a]
-        for a2, b2, j, w2 in open_:
-            own = i == j and (a, b) == (a2, b2) and src[i].dtype == dst[i].dtype
-            if written != w2 and not own:
-                raise GvdHipError('%s: a result shares memory with a gradient that is not its own' % what)
-        open_.append((a, b, i, written))
+def _check_scattered(o, src, dst, what):
+    """`o`, a result with gaps that is written by way of a copy, lies apart from every other tensor of the call."""
+    first, last = o.data_ptr(), o.data_ptr() + (sum((n - 1) * s for n, s in zip(o.shape, o.stride())) + 1) * o.element_size()
+    for t in src + dst:
+        if t is not o and t.data_ptr() < last and first < t.data_ptr() + t.numel() * t.element_size():
+            raise GvdHipError('%s: a result of strides %s lies among other tensors of the call' % (what, o.stride()))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
