@@ -44,13 +44,37 @@ struct SelectArgs {
   float* out_scores; int64_t* parent; int64_t* word; uint8_t* out_finished;
 };
 
+template <int STEP> __device__ __forceinline__ u64 dpp_u64(u64 x) {
+  return (u64)gvd_dpp<STEP>((unsigned)x, 0u) | (u64)gvd_dpp<STEP>((unsigned)(x >> 32), 0u) << 32;
+}
+template <int STEP> __device__ __forceinline__ u64 max_step(u64 x) {
+  const u64 o = dpp_u64<STEP>(x);
+  return o > x ? o : x;
+}
+__device__ __forceinline__ u64 lane63(u64 x) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, 63) | (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), 63) << 32;
+}
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const u64 o = __shfl_xor(v, off, GVD_WAVE);
-    v = o > v ? o : v;
-  }
-  return v;
+  v = max_step<0>(v); v = max_step<1>(v); v = max_step<2>(v);
+  v = max_step<3>(v); v = max_step<4>(v); v = max_step<5>(v);
+  return lane63(v);
+}
+
+template <int STEP> __device__ __forceinline__ unsigned extreme_step(unsigned x, bool largest) {
+  const unsigned hi = gvd_dpp<STEP>(x, 0u), lo = gvd_dpp<STEP>(x, 0xffffffffu);
+  return largest ? max(x, hi) : min(x, lo);
+}
+__device__ __forceinline__ float wave_max_f32(float f) {
+  unsigned x = order_bits(f);
+  x = extreme_step<0>(x, true); x = extreme_step<1>(x, true); x = extreme_step<2>(x, true);
+  x = extreme_step<3>(x, true); x = extreme_step<4>(x, true); x = extreme_step<5>(x, true);
+  return from_order_bits((unsigned)__builtin_amdgcn_readlane((int)x, 63));
+}
+// the smallest of the maxima of W or more equal groups of lanes: at least W lanes are at or over it
+__device__ __forceinline__ unsigned group_bound(unsigned x, int W) {
+  x = extreme_step<0>(x, 2 * W <= 64); x = extreme_step<1>(x, 4 * W <= 64); x = extreme_step<2>(x, 8 * W <= 64);
+  x = extreme_step<3>(x, 16 * W <= 64); x = extreme_step<4>(x, 32 * W <= 64); x = extreme_step<5>(x, 64 * W <= 64);
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 __device__ __forceinline__ int lanes_below(u64 mask, int lane) { return __popcll(mask & ((1ull << lane) - 1ull)); }
@@ -86,7 +110,7 @@ __device__ __forceinline__ void rank_list(u64* list, int n, int W, int lane) {
 // the first tile: with the lanes in W or more equal groups, the smallest of the groups' maxima is reached by W words.  The list is
 // ranked, and the floor raised, when it is full; logits of any order and equality only make that more frequent.
 template <typename T, int IPT>
-__global__ __launch_bounds__(256) void beam_part_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 && sizeof(T) == 2 ? 4 : 3))) void beam_part_kernel(const SelectArgs a) {
   constexpr int N = 16 / (int)sizeof(T), VECS = IPT / N, TILE = 64 * IPT;
   typedef typename GvdVec<T, N>::type Vec;
   typedef typename GvdVec<T, N>::loose Loose;
@@ -94,7 +118,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(const SelectArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int part = blockIdx.x * 4 + wave, row = blockIdx.y;
   if (part >= a.parts) return;
-  const bool skip = (a.finished && a.finished[row]) || !(fabsf(a.scores[row]) < INFINITY);
+  const float score = a.scores[row];
+  const bool over = a.finished ? a.finished[row] != 0 : false;
   const int W = a.W, V = a.V;
   const T* x = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld;
   u64* list = s_list[wave];
@@ -117,8 +142,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(const SelectArgs a) {
       }
     }
   };
-  if (skip) return;
-  fetch(first);
+  fetch(first);                            // (on its way while the beam's score is)
+  if (over || !(fabsf(score) < INFINITY)) return;
   for (int64_t v0 = first; v0 < end; v0 += TILE) {
     float v[IPT];
     float mx = -INFINITY;
@@ -133,47 +158,37 @@ __global__ __launch_bounds__(256) void beam_part_kernel(const SelectArgs a) {
 #pragma unroll
     for (int i = 0; i < IPT; ++i) s[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * 1.44269504088896341f);
     sum = sum * (double)__builtin_amdgcn_exp2f((was - ref) * 1.44269504088896341f) + (double)((s[0] + s[1]) + (s[2] + s[3]));
-    const unsigned ub = order_bits(mx);
-    if (v0 == first) {
-      unsigned g = ub;
-      int off = 1;
-      for (; off * 2 * W <= 64; off *= 2) g = max(g, (unsigned)__shfl_xor((int)g, off, GVD_WAVE));
-      for (; off < 64; off *= 2) g = min(g, (unsigned)__shfl_xor((int)g, off, GVD_WAVE));
-      floor = (u64)g << 32;
-    }
-    if (!__ballot(ub >= (unsigned)(floor >> 32))) continue;
+    if (v0 == first) floor = (u64)group_bound(order_bits(mx), W) << 32;
+    const float least = floor >> 32 ? from_order_bits((unsigned)(floor >> 32)) : -INFINITY;   // no word under it is among the best
+    if (!__ballot(mx >= least)) continue;
+    unsigned todo = 0;                     // the lane's words at or over it
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) {
-      const int64_t at = v0 + ((i / N) * 64 + lane) * N + i % N;
-      const u64 key = make_key(order_bits(v[i]), (int)at);
-      const bool hit = key >= floor && at < V;
-      const u64 hits = __ballot(hit);
-      if (hits) {
-        const int c = __popcll(hits);
-        if (n + c > LIST) {
-          wave_lds_fence();
-          rank_list(list, n, W, lane);
-          n = W;
-          floor = list[W - 1] > floor ? list[W - 1] : floor;
-        }
-        if (hit) list[n + lanes_below(hits, lane)] = key;
-        n += c;
+    for (int i = 0; i < IPT; ++i) todo |= v[i] >= least ? 1u << i : 0u;
+    while (true) {
+      const u64 any = __ballot(todo != 0);
+      if (!any || n + __popcll(any) > LIST) {
+        wave_lds_fence();
+        if (n > W) rank_list(list, n, W, lane);
+        n = W;
+        floor = list[W - 1] > floor ? list[W - 1] : floor;
+        if (!any) break;
       }
-    }
-    if (v0 + TILE < end && n > W) {
-      wave_lds_fence();
-      rank_list(list, n, W, lane);
-      n = W;
-      floor = list[W - 1] > floor ? list[W - 1] : floor;
+      const int i = __ffs(todo) - 1;       // the lane's next one (-1: none)
+      float mine = 0.f;
+#pragma unroll
+      for (int k = 0; k < IPT; ++k) mine = i == k ? v[k] : mine;
+      const int64_t at = v0 + ((i / N) * 64 + lane) * N + i % N;
+      const u64 key = make_key(order_bits(mine), (int)at);
+      const bool hit = todo && key >= floor && at < V;
+      const u64 hits = __ballot(hit);
+      if (hit) list[n + lanes_below(hits, lane)] = key;
+      n += __popcll(hits);
+      todo &= todo - 1;
     }
   }
-  wave_lds_fence();
-  if (n > W) rank_list(list, n, W, lane);
   // the lanes' sums, each to its own maximum, into one (NaN and +inf go through to the join, which drops the beam)
-  const float all = wave_max(top);
-  sum = sum != 0.0 ? sum * exp((double)top - (double)all) : 0.0;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, GVD_WAVE);
+  const float all = wave_max_f32(top);
+  sum = gvd_wave_sum_f64(sum != 0.0 ? sum * (double)__builtin_amdgcn_exp2f((top - all) * 1.44269504088896341f) : 0.0);
   const int64_t rec = (int64_t)row * a.parts + part;
   if (lane == 0) a.stat[rec] = make_double2((double)all, sum);
   if (lane < W) a.best[rec * W + lane] = list[lane];
@@ -194,7 +209,16 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
     double* score_q = s_score + q * W;
     int* word_q = s_word + q * W;
     const float score = a.scores[row];
-    const bool over = a.finished && a.finished[row];
+    const bool over = a.finished ? a.finished[row] != 0 : false;
+    // (loaded before they are known to be there: the lists of a beam that was passed over hold anything, and are not used)
+    const int64_t rec = (int64_t)row * a.parts;
+    const int total = a.parts * W;
+    const u64* words = a.best + rec * W;
+    const double2 st = lane < a.parts ? a.stat[rec + lane] : make_double2(-INFINITY, 0.0);
+    u64 floor = lane < a.parts ? words[lane * W + W - 1] : 0;
+    u64 mine[JOIN_LIST / 64];
+#pragma unroll
+    for (int i = 0; i < JOIN_LIST / 64; ++i) mine[i] = lane + 64 * i < total ? words[lane + 64 * i] : 0;
     bool live = fabsf(score) < INFINITY;
     if (live && over) {
       if (lane < W) {
@@ -205,23 +229,9 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
       continue;
     }
     double lse = 0.0;
-    u64 mine[JOIN_LIST / 64];
-    u64 floor = 0;
-    const int total = a.parts * W;
     if (live) {
-      const int64_t rec = (int64_t)row * a.parts;
-      const double2 st = lane < a.parts ? a.stat[rec + lane] : make_double2(-INFINITY, 0.0);
-      const u64* list = a.best + rec * W;
-      floor = lane < a.parts ? list[lane * W + W - 1] : 0;
-#pragma unroll
-      for (int i = 0; i < JOIN_LIST / 64; ++i) mine[i] = lane + 64 * i < total ? list[lane + 64 * i] : 0;
-      double m = st.x;
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) m = fmax(m, __shfl_xor(m, off, GVD_WAVE));
-      double s = lane < a.parts && st.y != 0.0 ? st.y * exp(st.x - m) : 0.0;
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, GVD_WAVE);
-      lse = m + log(s);
+      const double m = wave_max_f32((float)st.x);
+      lse = m + log(gvd_wave_sum_f64(lane < a.parts && st.y != 0.0 ? st.y * exp(st.x - m) : 0.0));
       live = fabs(lse) < INFINITY;
     }
     if (!live) {
@@ -320,14 +330,13 @@ bool bad_select_shape(int B, int K, int V, int W) {
 // ------------------------------------------------------------------------------------------------------------- reorder
 // dst[o, r, :] = src[o, index[r], :], up to GVD_REORDER_MAX_TENSORS tensors in a launch.  A copy: bound by reading and writing
 // the rows once.  A thread copies four units of 16 bytes; the last unit of a row is moved back so that it ends with the row
-// (rows under 16 bytes: units of the largest power of two that divides them).
+// (rows under 16 bytes: units of 8, 4 or 1 bytes).
 constexpr int UNITS = 1024;               // units of one workgroup
 
 template <int BYTES> struct Unit;
 template <> struct Unit<16> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(1))); };
 template <> struct Unit<8> { typedef unsigned type __attribute__((ext_vector_type(2), aligned(1))); };
 template <> struct Unit<4> { typedef unsigned type __attribute__((aligned(1))); };
-template <> struct Unit<2> { typedef uint16_t type __attribute__((aligned(1))); };
 template <> struct Unit<1> { typedef uint8_t type; };
 
 template <int BYTES>
@@ -345,13 +354,12 @@ __device__ void reorder_tile(const gvd_reorder_tensor& t, const int64_t* __restr
     src[u] = from >= 0 && from < rows_in ? reinterpret_cast<const char*>(t.src) + o * t.src_outer + from * t.src_row + off : nullptr;
   };
   if (per_row >= UNITS) {                 // a tile lies in one row (the host counts tiles the same way)
-    const int64_t tiles = (per_row + UNITS - 1) / UNITS;
-    const int64_t row = tile / tiles, o = row / rows_out;
-    const int64_t unit0 = (tile - row * tiles) * UNITS + threadIdx.x;
+    const unsigned tiles = (unsigned)((per_row + UNITS - 1) / UNITS), row = (unsigned)tile / tiles, o = row / (unsigned)rows_out;
+    const int64_t unit0 = (int64_t)((unsigned)tile - row * tiles) * UNITS + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       dst[u] = nullptr; src[u] = nullptr;
-      if (unit0 + 256 * u < per_row) place(u, o, row - o * rows_out, unit0 + 256 * u);
+      if (unit0 + 256 * u < per_row) place(u, o, row - o * (unsigned)rows_out, unit0 + 256 * u);
     }
   } else {                                // (fewer than 2^31 units: 32-bit divisions)
     const unsigned total = (unsigned)(t.outer * rows_out * per_row), pr = (unsigned)per_row, ro = (unsigned)rows_out;
@@ -386,7 +394,6 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(const gvd_reorder_gro
     case 16: reorder_tile<16>(x, index, rows_in, rows_out, tile); break;
     case 8: reorder_tile<8>(x, index, rows_in, rows_out, tile); break;
     case 4: reorder_tile<4>(x, index, rows_in, rows_out, tile); break;
-    case 2: reorder_tile<2>(x, index, rows_in, rows_out, tile); break;
     default: reorder_tile<1>(x, index, rows_in, rows_out, tile); break;
   }
 }
@@ -440,8 +447,7 @@ extern "C" int gvd_reorder_rows(const gvd_reorder_group* group, const int64_t* i
   for (int i = 0; i < g.count; ++i) {
     gvd_reorder_tensor& t = g.t[i];
     if (!t.src || !t.dst || t.outer <= 0 || t.outer > 0x7fffffffll || t.row_bytes <= 0) return GVD_EINVAL;
-    t.unit = 16;
-    while (t.unit > 1 && (t.row_bytes < t.unit || (t.row_bytes < 16 && t.row_bytes % t.unit))) t.unit /= 2;
+    t.unit = t.row_bytes >= 16 ? 16 : t.row_bytes % 8 == 0 ? 8 : t.row_bytes % 4 == 0 ? 4 : 1;
     g.tile0[i] = tiles;
     const int64_t per_row = (t.row_bytes + t.unit - 1) / t.unit;
     if (t.outer > (1ll << 33) / rows_out || per_row > (1ll << 33) / (t.outer * rows_out)) return GVD_EINVAL;

@@ -22,18 +22,25 @@ __device__ __forceinline__ unsigned wave_id() {
   return __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));          // (workgroups of four waves)
 }
 
+// A lane's first column in slice `slice` of 64 * N columns; -1: none.  The last lane of a row is moved back so that it ends with the
+// row: it does some of its neighbour's columns again, the same sums in the same order, instead of a part of a vector (host: the
+// width is N at least).
+template <int N> __device__ __forceinline__ int lane_column(unsigned slice, int width) {
+  const int col = (int)(slice * 64 + (threadIdx.x & 63)) * N;
+  return col >= width ? -1 : col <= width - N ? col : width - N;
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
 // One wave per R rows and 64 * N columns (a slice); the R tokens, then the R rows, are on their way together.  Waves next to each
 // other take the slices of the same rows, so that a row is one stretch of memory traffic.
-template <typename T, int N, int R>
+template <typename T, int N, int R, bool PAST>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int tok64, int64_t n, const T* __restrict__ table,
                                                             int64_t ld, unsigned vocab, int width, float scale, int act,
                                                             T* __restrict__ out, int64_t ldo, unsigned slices) {
   const unsigned id = wave_id(), unit = id / slices;
   const int64_t row0 = (int64_t)unit * R;
-  const int col = ((int)(id - unit * slices) * 64 + (threadIdx.x & 63)) * N;
-  if (row0 >= n || col >= width) return;
-  const int left = width - col;
+  const int col = lane_column<N>(id - unit * slices, width);
+  if (row0 >= n || col < 0) return;
   unsigned v[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) v[r] = row0 + r < n ? token_key(tok, tok64, row0 + r, vocab, -1) : vocab;
@@ -44,8 +51,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int
 #pragma unroll
       for (int k = 0; k < N; ++k) x[r][k] = __builtin_nanf("");
     } else {
-      const T* w = table + (int64_t)v[r] * ld + col;
-      if (left >= N) gvd_load<T, N>(w, x[r]); else gvd_load_part<T, N>(w, left, x[r]);
+      gvd_load<T, N>(table + (int64_t)v[r] * ld + col, x[r]);
     }
   }
 #pragma unroll
@@ -57,7 +63,8 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int
       if (act) x[r][k] = act_relu(x[r][k]);
     }
     T* o = out + (row0 + r) * ldo + col;
-    if (left >= N) gvd_store<T, N>(o, x[r]); else gvd_store_part<T, N>(o, left, x[r]);
+    if constexpr (PAST) gvd_store_past<T, N>(o, x[r]);
+    else gvd_store<T, N>(o, x[r]);
   }
 }
 
@@ -105,8 +112,8 @@ __global__ __launch_bounds__(RANK_THREADS) void token_rank_kernel(const void* to
 }
 
 // Larger n: stable counting sorts by digits of up to 9 bits, least significant first.  The positions are cut into at most
-// SORT_BLOCKS contiguous parts, one workgroup each: a launch counts every part's digits, the next one places them - each
-// workgroup adds up the counts before its own by itself.  A wave takes 64 consecutive positions at a time; lanes of equal digit
+// SORT_BLOCKS contiguous parts, one workgroup each: a launch counts every part's digits, the next one places them, each
+// workgroup adding up the counts before its own by itself.  A wave takes 64 consecutive positions at a time; lanes of equal digit
 // find each other by ballots, so equal digits keep their order.
 constexpr int SORT_BLOCKS = 128;
 constexpr int SORT_BITS = 9;
@@ -117,7 +124,7 @@ struct SortPass {
   const void* tok; int tok64; unsigned vocab; int64_t pad;       // first pass: keys from the tokens, positions 0, 1, ...
   const unsigned* key_in; const unsigned* pos_in;                // later passes
   unsigned* key_out; unsigned* pos_out;
-  unsigned* hist;                                                // [blocks][SORT_DIGITS]
+  unsigned* hist;                                                // [parts][SORT_DIGITS]
   int64_t n, per;                                                // positions; positions of one workgroup
   int shift, bits;
 };
@@ -139,17 +146,36 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const SortPass p) {
 
 __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
   __shared__ unsigned s_next[SORT_DIGITS];                   // where the next position of this digit goes
-  __shared__ unsigned s_wave[4][SORT_DIGITS];
+  __shared__ __attribute__((aligned(16))) unsigned s_wave[4][SORT_DIGITS];
+  __shared__ __attribute__((aligned(16))) unsigned s_all[4][SORT_DIGITS];
   __shared__ unsigned s_sum[4];
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const unsigned mask = (1u << p.bits) - 1;
-  // digits 2 tid, 2 tid + 1: their counts before this part, and in all
-  unsigned before[2] = {0, 0}, all[2] = {0, 0};
+  const int64_t i0 = (int64_t)blockIdx.x * p.per, i1 = i0 + p.per < p.n ? i0 + p.per : p.n;
+  // counts of every digit before this part, and in all: a wave adds up every fourth part, a lane 8 digits
+  {
+    u32x4 before[2] = {}, all[2] = {};
 #pragma unroll 8
-  for (unsigned b = 0; b < gridDim.x; ++b) {
-    const uint2 h = *reinterpret_cast<const uint2*>(p.hist + (int64_t)b * SORT_DIGITS + 2 * tid);
-    all[0] += h.x; all[1] += h.y;
-    if (b < blockIdx.x) { before[0] += h.x; before[1] += h.y; }
+    for (unsigned b = wave; b < gridDim.x; b += 4) {
+      const u32x4* h = reinterpret_cast<const u32x4*>(p.hist + (int64_t)b * SORT_DIGITS + 8 * lane);
+      const u32x4 x = h[0], y = h[1];
+      all[0] += x; all[1] += y;
+      if (b < blockIdx.x) { before[0] += x; before[1] += y; }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      *reinterpret_cast<u32x4*>(&s_wave[wave][8 * lane + 4 * k]) = before[k];
+      *reinterpret_cast<u32x4*>(&s_all[wave][8 * lane + 4 * k]) = all[k];
+    }
+  }
+  __syncthreads();
+  unsigned before[2], all[2];                                // digits 2 tid, 2 tid + 1
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = 2 * tid + k;
+    before[k] = s_wave[0][d] + s_wave[1][d] + s_wave[2][d] + s_wave[3][d];
+    all[k] = s_all[0][d] + s_all[1][d] + s_all[2][d] + s_all[3][d];
   }
   unsigned upto = all[0] + all[1];
 #pragma unroll
@@ -163,15 +189,18 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
   for (int w = 0; w < wave; ++w) base += s_sum[w];
   s_next[2 * tid] = base + before[0];
   s_next[2 * tid + 1] = base + all[0] + before[1];
-  const int64_t i0 = (int64_t)blockIdx.x * p.per, i1 = i0 + p.per < p.n ? i0 + p.per : p.n;
   constexpr int ROUNDS = SORT_TILE / 256;
   for (int64_t t0 = i0; t0 < i1; t0 += SORT_TILE) {
     for (int d = tid; d < 4 * SORT_DIGITS; d += 256) (&s_wave[0][0])[d] = 0;
-    __syncthreads();
-    unsigned key[ROUNDS], place[ROUNDS];
+    unsigned key[ROUNDS], pos[ROUNDS], place[ROUNDS];
     const int64_t w0 = t0 + wave * (SORT_TILE / 4) + lane;
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) key[r] = w0 + 64 * r < i1 ? sort_key(p, w0 + 64 * r) : 0;
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int64_t i = w0 + 64 * r;
+      key[r] = i < i1 ? sort_key(p, i) : 0;
+      pos[r] = i < i1 && !p.tok ? p.pos_in[i] : (unsigned)i;
+    }
+    __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const bool in = w0 + 64 * r < i1;
@@ -191,18 +220,19 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-      const int64_t i = w0 + 64 * r;
-      if (i < i1) {
+      if (w0 + 64 * r < i1) {
         const unsigned d = (key[r] >> p.shift) & mask;
         unsigned to = s_next[d] + place[r];
         for (int w = 0; w < wave; ++w) to += s_wave[w][d];
         p.key_out[to] = key[r];
-        p.pos_out[to] = p.tok ? (unsigned)i : p.pos_in[i];
+        p.pos_out[to] = pos[r];
       }
     }
-    __syncthreads();
-    for (int d = tid; d < SORT_DIGITS; d += 256) s_next[d] += s_wave[0][d] + s_wave[1][d] + s_wave[2][d] + s_wave[3][d];
-    __syncthreads();
+    if (t0 + SORT_TILE < i1) {
+      __syncthreads();
+      for (int d = tid; d < SORT_DIGITS; d += 256) s_next[d] += s_wave[0][d] + s_wave[1][d] + s_wave[2][d] + s_wave[3][d];
+      __syncthreads();
+    }
   }
 }
 
@@ -222,32 +252,22 @@ struct SumArgs {
   unsigned slices; int stretch;
 };
 
-// A lane's columns of a row: N of them, the last lane of a row fewer, the lanes behind it none.
-template <typename T, int N> struct Columns {
-  int col, left;
-  typedef typename GvdVec<T, N>::type Raw;       // (as loaded: rows in flight cost half the registers in 16-bit types)
-  __device__ __forceinline__ Raw fetch(const T* row) const {
-    if (left >= N) return *reinterpret_cast<const typename GvdVec<T, N>::loose*>(row + col);
-    Raw x;
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = k < left ? row[col + k] : (T)0;
-    return x;
-  }
-  __device__ __forceinline__ void store(T* row, const float (&x)[N]) const {
-    if (left >= N) gvd_store<T, N>(row + col, x); else gvd_store_part<T, N>(row + col, left, x);
-  }
-};
+// a lane's N columns of a row, as loaded (rows in flight cost half the registers in 16-bit types)
+template <typename T, int N> __device__ __forceinline__ typename GvdVec<T, N>::type fetch(const T* row, int col) {
+  if (col < 0) return {};
+  return *reinterpret_cast<const typename GvdVec<T, N>::loose*>(row + col);
+}
 
 // s += `count` (<= 64) rows of x, in order: row i is the one that lane i names (`which`); FLIGHT bytes of a lane on their way at
 // a time, 16 rows at most
 template <typename T, int N, int FLIGHT>
-__device__ __forceinline__ void add_rows(const T* x, int64_t ld, unsigned which, int count, const Columns<T, N>& c, float (&s)[N]) {
+__device__ __forceinline__ void add_rows(const T* x, int64_t ld, unsigned which, int count, int col, float (&s)[N]) {
   constexpr int BATCH = FLIGHT / (int)(sizeof(T) * N) < 16 ? FLIGHT / (int)(sizeof(T) * N) : 16;
   for (int i = 0; i < count; i += BATCH) {
-    typename Columns<T, N>::Raw r[BATCH];
+    typename GvdVec<T, N>::type r[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k)
-      if (i + k < count) r[k] = c.fetch(x + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, i + k) * ld);
+      if (i + k < count) r[k] = fetch<T, N>(x + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, i + k) * ld, col);
 #pragma unroll
     for (int k = 0; k < BATCH; ++k)
       if (i + k < count) {
@@ -257,21 +277,11 @@ __device__ __forceinline__ void add_rows(const T* x, int64_t ld, unsigned which,
   }
 }
 
-// s += dy rows of the sorted positions [i, e)
-template <typename T, int N>
-__device__ __forceinline__ void add_positions(const SumArgs& a, int64_t i, int64_t e, int lane, const Columns<T, N>& c, float (&s)[N]) {
-  for (; i < e; i += 64) {
-    const unsigned which = i + lane < e ? a.spos[i + lane] : 0;
-    add_rows<T, N, 128>(reinterpret_cast<const T*>(a.dy), a.ld, which, e - i < 64 ? (int)(e - i) : 64, c, s);
-  }
-}
-
 // s += rows [i, e) of partial sums
 template <int N>
-__device__ __forceinline__ void add_partials(const float* part, int width, int64_t i, int64_t e, int lane, const Columns<float, N>& c,
-                                             float (&s)[N]) {
+__device__ __forceinline__ void add_partials(const float* part, int width, int64_t i, int64_t e, int col, float (&s)[N]) {
   for (; i < e; i += 64)
-    add_rows<float, N, 128>(part + i * width, width, (unsigned)lane, e - i < 64 ? (int)(e - i) : 64, c, s);
+    add_rows<float, N, 128>(part + i * width, width, threadIdx.x & 63, e - i < 64 ? (int)(e - i) : 64, col, s);
 }
 
 // level 1: whole groups of 32 positions of a token with 64 positions or more; level 2: whole groups of 32 such groups
@@ -282,11 +292,10 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
   constexpr int64_t LEN = LEVEL == 1 ? GROUP : GROUP * GROUP;
   const int64_t i0 = (int64_t)g * LEN;
   if (i0 + LEN > a.n) return;
-  const int col = ((int)(id - g * a.slices) * 64 + lane) * N;
+  const int col = lane_column<N>(id - g * a.slices, a.width);
   float s[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) s[k] = 0.f;
-  const Columns<float, N> cf = {col, a.width - col};
   if constexpr (LEVEL == 1) {
     // keys of [i0 - 32, i0 + 64): the group, and 32 more of the same on its two sides together - else the token has fewer than 64
     const int64_t b = i0 - 32 + lane, e = i0 + 32 + lane;
@@ -295,13 +304,13 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
     const unsigned v = __builtin_amdgcn_readlane(before, 32);
     if (v >= a.vocab || __builtin_amdgcn_readlane(before, 63) != v) return;
     if (__popcll(__ballot(before == v)) + __popcll(__ballot(after == v)) < 64) return;
-    add_rows<T, N, 256>(reinterpret_cast<const T*>(a.dy), a.ld, which, GROUP, Columns<T, N>{col, a.width - col}, s);
+    add_rows<T, N, 256>(reinterpret_cast<const T*>(a.dy), a.ld, which, GROUP, col, s);
   } else {
     const unsigned v = a.skey[i0], last = a.skey[i0 + LEN - 1];
     if (v >= a.vocab || last != v) return;
-    add_rows<float, N, 256>(a.part1 + (int64_t)g * GROUP * a.width, a.width, (unsigned)lane, GROUP, cf, s);
+    add_rows<float, N, 256>(a.part1 + (int64_t)g * GROUP * a.width, a.width, (unsigned)lane, GROUP, col, s);
   }
-  cf.store((LEVEL == 1 ? a.part1 : a.part2) + (int64_t)g * a.width, s);
+  if (col >= 0) gvd_store<float, N>((LEVEL == 1 ? a.part1 : a.part2) + (int64_t)g * a.width + col, s);
 }
 
 // first sorted position i in [lo, n) with skey[i] >= v (RISE = 0), or skey[i] + i >= v (RISE = 1): 64 lanes look at 64 places at
@@ -328,14 +337,13 @@ __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_
 // stretch (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows
 // without a position as zeros.  So no wave has much more to do than another, whatever the tokens are.  It walks 64 sorted
 // positions at a time; the dy rows of several tokens are on their way together.
-template <typename T, int N>
+template <typename T, int N, bool PAST>
 __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
   const unsigned id = wave_id(), unit = id / a.slices;
   const int lane = threadIdx.x & 63;
   const int64_t d0 = (int64_t)unit * a.stretch, d1 = d0 + a.stretch;
   if (d0 >= (int64_t)a.vocab + a.n) return;
-  const int col = ((int)(id - unit * a.slices) * 64 + lane) * N;
-  const Columns<T, N> c = {col, a.width - col};
+  const int col = lane_column<N>(id - unit * a.slices, a.width);
   const T* dy = reinterpret_cast<const T*>(a.dy);
   T* dw = reinterpret_cast<T*>(a.dw);
   float s[N];
@@ -352,27 +360,28 @@ __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
   } else if (i > 0 && i == a.n && a.skey[i - 1] == cur) {
     ++cur;
   }
-  const auto zeros = [&](int64_t to) {           // rows cur ... to - 1 have no positions
+  const auto put = [&](unsigned v, const float (&x)[N]) {
+    if (col < 0) return;
+    T* o = dw + (int64_t)v * a.width + col;
+    if constexpr (PAST) gvd_store_past<T, N>(o, x); else gvd_store<T, N>(o, x);
+  };
+  // rows cur ... v - 1 have no positions; row v, where there is a sum for it, is s
+  const auto finish = [&](int64_t v, bool sum) {
     float x[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) x[k] = 0.f;
-    for (; (int64_t)cur < to; ++cur)
-      if (c.left > 0) c.store(dw + (int64_t)cur * a.width, x);
-  };
-  const auto finish = [&](unsigned v) {          // row v is s
-    if (c.left > 0) {
-      float x[N];
-      if (a.act) {
-        const typename Columns<T, N>::Raw w = c.fetch(reinterpret_cast<const T*>(a.table) + (int64_t)v * a.ldt);
+    for (; (int64_t)cur < v; ++cur) put(cur, x);
+    if (!sum) return;
+    if (a.act) {
+      const typename GvdVec<T, N>::type w = fetch<T, N>(reinterpret_cast<const T*>(a.table) + v * a.ldt, col);
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = (float)w[k] * a.scale > 0.f ? s[k] * a.scale : 0.f;
-      } else {
+      for (int k = 0; k < N; ++k) x[k] = (float)w[k] * a.scale > 0.f ? s[k] * a.scale : 0.f;
+    } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = s[k] * a.scale;
-      }
-      c.store(dw + (int64_t)v * a.width, x);
+      for (int k = 0; k < N; ++k) x[k] = s[k] * a.scale;
     }
-    cur = v + 1;
+    put((unsigned)v, x);
+    cur = (unsigned)v + 1;
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = 0.f;
   };
@@ -380,23 +389,21 @@ __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
     const unsigned key = i + lane < a.n ? a.skey[i + lane] : a.vocab;
     const unsigned which = i + lane < a.n ? a.spos[i + lane] : 0;
     const unsigned first = __builtin_amdgcn_readfirstlane(key), last = __builtin_amdgcn_readlane(key, 63);
-    zeros((int64_t)first < d1 - i ? (int64_t)first : d1 - i);
+    finish((int64_t)first < d1 - i ? (int64_t)first : d1 - i, false);
     if (first >= a.vocab || (int64_t)first >= d1 - i) break;
     if (first == last) {                         // 64 positions or more of one token
       const int64_t e = wave_lower_bound<0>(a.skey, i + 64, a.n, first + 1, lane);
       const int64_t g1 = (i + GROUP - 1) / GROUP, g2 = e / GROUP;                 // whole groups (there is one at least)
-      const Columns<float, N> cf = {c.col, c.left};
-      add_positions<T, N>(a, i, g1 * GROUP, lane, c, s);
+      const int head = (int)(g1 * GROUP - i), ends = head + (int)(e - g2 * GROUP);  // positions before and behind them
+      const int64_t at = lane < head ? i + lane : g2 * GROUP + lane - head;
+      add_rows<T, N, 128>(dy, a.ld, lane < ends ? a.spos[at] : 0, ends, col, s);
       const int64_t h1 = (g1 + GROUP - 1) / GROUP, h2 = g2 / GROUP;               // whole groups of groups
-      if (a.n < LEVEL2_FROM || h1 >= h2) {
-        add_partials<N>(a.part1, a.width, g1, g2, lane, cf, s);
-      } else {
-        add_partials<N>(a.part1, a.width, g1, h1 * GROUP, lane, cf, s);
-        add_partials<N>(a.part2, a.width, h1, h2, lane, cf, s);
-        add_partials<N>(a.part1, a.width, h2 * GROUP, g2, lane, cf, s);
+      const bool two = a.n >= LEVEL2_FROM && h1 < h2;
+      for (int k = 0; k < 3; ++k) {              // groups before, groups of groups, groups behind them
+        const int64_t from = k == 0 ? g1 : k == 1 ? h1 : two ? h2 * GROUP : g2, to = k == 0 ? (two ? h1 * GROUP : g2) : k == 1 ? (two ? h2 : h1) : g2;
+        add_partials<N>(k == 1 ? a.part2 : a.part1, a.width, from, to, col, s);
       }
-      add_positions<T, N>(a, g2 * GROUP, e, lane, c, s);
-      finish(first);
+      finish(first, true);
       i = e;
       continue;
     }
@@ -405,22 +412,19 @@ __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
     const unsigned long long behind = __ballot((lane == 0 || key != left) && (key >= a.vocab || (int64_t)key + i + lane >= d1));
     int count = __popcll(__ballot(key != last));
     if (behind) count = count < __ffsll(behind) - 1 ? count : __ffsll(behind) - 1;
-    constexpr int BATCH = 8;
+    constexpr int BATCH = 4;
     for (int j0 = 0; j0 < count; j0 += BATCH) {
-      typename Columns<T, N>::Raw x[BATCH];
+      typename GvdVec<T, N>::type x[BATCH];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k)
-        if (j0 + k < count) x[k] = c.fetch(dy + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, j0 + k) * a.ld);
+        if (j0 + k < count) x[k] = fetch<T, N>(dy + (int64_t)(unsigned)__builtin_amdgcn_readlane(which, j0 + k) * a.ld, col);
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
         if (j0 + k < count) {
           const unsigned v = __builtin_amdgcn_readlane(key, j0 + k);
 #pragma unroll
           for (int e = 0; e < N; ++e) s[e] += (float)x[k][e];
-          if (__builtin_amdgcn_readlane(key, j0 + k + 1) != v) {                  // (count <= 63: lane 63 belongs to a later token)
-            zeros(v);
-            finish(v);
-          }
+          if (__builtin_amdgcn_readlane(key, j0 + k + 1) != v) finish(v, true);   // (count <= 63: lane 63 belongs to a later token)
         }
       }
     }
@@ -485,7 +489,8 @@ int launch_fwd(const void* tok, int tok64, int64_t n, const void* table, int64_t
   const bool many = n * slices >= 16384;   // (four rows a wave still leave four waves to every SIMD)
   const int64_t waves = (many ? (n + 3) / 4 : n) * slices;
   if (waves > MAX_WAVES) return GVD_EINVAL;
-  hipLaunchKernelGGL((many ? embedding_fwd_kernel<T, N, 4> : embedding_fwd_kernel<T, N, 1>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
+  const bool past = n * width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
+  hipLaunchKernelGGL((!many ? embedding_fwd_kernel<T, N, 1, false> : past ? embedding_fwd_kernel<T, N, 4, true> : embedding_fwd_kernel<T, N, 4, false>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
                      st, tok, tok64, n, reinterpret_cast<const T*>(table), ld, (unsigned)vocab, width, scale, act,
                      reinterpret_cast<T*>(out), ldo, slices);
   GVD_CHECK_LAUNCH();
@@ -507,7 +512,8 @@ template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
     hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
     GVD_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL((token_rows_kernel<T, N>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
+  const bool past = (int64_t)a.vocab * a.width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
+  hipLaunchKernelGGL((past ? token_rows_kernel<T, N, true> : token_rows_kernel<T, N, false>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
   GVD_CHECK_LAUNCH();
   return 0;
 }

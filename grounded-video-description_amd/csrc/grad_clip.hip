@@ -84,19 +84,23 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(const gvd_grad_group g,
 // the factor as a product of two: one that fp32 holds as a normal number, and a power of two (1 but for norms over 2^100)
 struct Factor { float f, p; };
 
-template <typename TI, typename TO> __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, Factor f) {
+template <bool PAST, typename TI, typename TO>
+__device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, Factor f) {
   constexpr int N = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO)), VECS = CHUNK / (256 * N);
   if (n == CHUNK) {
     typename GvdVec<TI, N>::type x[VECS];
 #pragma unroll
-    for (int i = 0; i < VECS; ++i)
-      x[i] = *reinterpret_cast<const typename GvdVec<TI, N>::loose*>(src + (i * 256 + threadIdx.x) * N);
+    for (int i = 0; i < VECS; ++i) {
+      const auto* from = reinterpret_cast<const typename GvdVec<TI, N>::loose*>(src + (i * 256 + threadIdx.x) * N);
+      if constexpr (PAST) x[i] = __builtin_nontemporal_load(from); else x[i] = *from;
+    }
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       float v[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) v[k] = (float)x[i][k] * f.f * f.p;
-      gvd_store<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
+      if constexpr (PAST) gvd_store_past<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
+      else gvd_store<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
     }
     return;
   }
@@ -111,12 +115,24 @@ template <typename TI, typename TO> __device__ __forceinline__ void chunk_scale(
   for (int64_t i = nv + threadIdx.x; i < n; i += 256) dst[i] = (TO)((float)src[i] * f.f * f.p);
 }
 
-template <typename TI> __device__ __forceinline__ void scale_to(const TI* src, void* dst, int type, int64_t e0, int64_t n, Factor f) {
-  if (type == GVD_F32) chunk_scale(src + e0, reinterpret_cast<float*>(dst) + e0, n, f);
-  else if (type == GVD_BF16) chunk_scale(src + e0, reinterpret_cast<gvd_bf16*>(dst) + e0, n, f);
-  else chunk_scale(src + e0, reinterpret_cast<gvd_f16*>(dst) + e0, n, f);
+// Chunk k of a tensor.  Its chunks begin where the destination begins a 128-byte line (the first one holds what lies before, too):
+// results that are views of a flat buffer begin anywhere, and stores of parts of lines cost more than such loads.
+template <bool PAST, typename TI, typename TO>
+__device__ __forceinline__ void scale_chunk(const TI* src, TO* dst, int64_t k, int64_t n, Factor f) {
+  const int64_t before = (int64_t)((128u - (unsigned)(reinterpret_cast<uintptr_t>(dst) & 127u)) % 128u / sizeof(TO));
+  if (k == 0 && threadIdx.x < before && threadIdx.x < n) dst[threadIdx.x] = (TO)((float)src[threadIdx.x] * f.f * f.p);
+  const int64_t e0 = k * CHUNK + before, e1 = e0 + CHUNK < n ? e0 + CHUNK : n;
+  if (e0 < e1) chunk_scale<PAST>(src + e0, dst + e0, e1 - e0, f);
 }
 
+template <bool PAST, typename TI>
+__device__ __forceinline__ void scale_to(const TI* src, void* dst, int type, int64_t k, int64_t n, Factor f) {
+  if (type == GVD_F32) scale_chunk<PAST>(src, reinterpret_cast<float*>(dst), k, n, f);
+  else if (type == GVD_BF16) scale_chunk<PAST>(src, reinterpret_cast<gvd_bf16*>(dst), k, n, f);
+  else scale_chunk<PAST>(src, reinterpret_cast<gvd_f16*>(dst), k, n, f);
+}
+
+template <bool PAST>
 __global__ __launch_bounds__(256) void grad_scale_kernel(const gvd_grad_group g, const gvd_grad_clip c,
                                                          const double* __restrict__ partials, int n_partials, float* norm_out) {
   __shared__ double s_red[4];
@@ -135,11 +151,11 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const gvd_grad_group g,
     const unsigned k = chunks - 1 - at;
     const int t = first.tensor_of(k);
     if (factor == 1.0 && g.src[t] == g.dst[t]) continue;                       // in place and nothing to clip
-    const int64_t e0 = (int64_t)(k - g.chunk0[t]) * CHUNK;
-    const int64_t n = g.n[t] - e0 < CHUNK ? g.n[t] - e0 : CHUNK;
-    if (g.src_type[t] == GVD_F32) scale_to(reinterpret_cast<const float*>(g.src[t]), g.dst[t], g.dst_type[t], e0, n, f);
-    else if (g.src_type[t] == GVD_BF16) scale_to(reinterpret_cast<const gvd_bf16*>(g.src[t]), g.dst[t], g.dst_type[t], e0, n, f);
-    else scale_to(reinterpret_cast<const gvd_f16*>(g.src[t]), g.dst[t], g.dst_type[t], e0, n, f);
+    const int64_t at_t = k - g.chunk0[t], n = g.n[t];
+    const int to = g.dst_type[t];
+    if (g.src_type[t] == GVD_F32) scale_to<PAST>(reinterpret_cast<const float*>(g.src[t]), g.dst[t], to, at_t, n, f);
+    else if (g.src_type[t] == GVD_BF16) scale_to<PAST>(reinterpret_cast<const gvd_bf16*>(g.src[t]), g.dst[t], to, at_t, n, f);
+    else scale_to<PAST>(reinterpret_cast<const gvd_f16*>(g.src[t]), g.dst[t], to, at_t, n, f);
   }
 }
 
@@ -181,9 +197,11 @@ extern "C" int gvd_grad_scale(const gvd_grad_group* g, const gvd_grad_clip* c, c
   if (bad_group(g, true) || !c || !(c->max_norm >= 0.0) || !(c->inv_scale > 0.0) || !partials || n_partials <= 0 ||
       reinterpret_cast<uintptr_t>(partials) % 8 || (g->count == 0 && !norm_out))
     return GVD_EINVAL;
-  const unsigned grid = g->count ? grid_of(g, 2 * MAX_GRID) : 1;
-  hipLaunchKernelGGL(grad_scale_kernel, dim3(grid), dim3(256), 0, gvd_s(stream), *g, *c,
-                     reinterpret_cast<const double*>(partials), n_partials, norm_out);
+  int64_t bytes = 0;
+  for (int t = 0; t < g->count; ++t) bytes += g->n[t] * (gvd_dtype_bytes(g->src_type[t]) + gvd_dtype_bytes(g->dst_type[t]));
+  const unsigned grid = g->count ? grid_of(g, 8 * MAX_GRID) : 1;
+  hipLaunchKernelGGL((bytes > GVD_CACHE_BYTES ? grad_scale_kernel<true> : grad_scale_kernel<false>), dim3(grid), dim3(256), 0,
+                     gvd_s(stream), *g, *c, reinterpret_cast<const double*>(partials), n_partials, norm_out);
   GVD_CHECK_LAUNCH();
   return 0;
 }

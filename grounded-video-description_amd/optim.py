@@ -149,7 +149,7 @@ class ClipAdam(torch.optim.Adam):
 # fp32, bf16 and fp16 gradients, mixed, clipped in place or written - unscaled - into master gradients of another type.  What
 # is looked at per tensor goes through map() and numpy: with hundreds of small gradients the host is what a call waits for.
 # ---------------------------------------------------------------------------------------------------------------------
-_DTYPE = operator.attrgetter('dtype')
+_DTYPE, _SHAPE = operator.attrgetter('dtype'), operator.attrgetter('shape')
 _T = torch.Tensor
 _GROUP_FIELDS = {f: (getattr(GradGroup, f).offset, t) for f, t in (('src', np.int64), ('dst', np.int64), ('n', np.int64),
                                                                    ('chunk0', np.uint32), ('src_type', np.uint8), ('dst_type', np.uint8))}
@@ -172,34 +172,40 @@ def _repeats(t):
     return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
 
 
-def _check_grads(grads, what):
-    """Dense float tensors on one GPU."""
-    for i, g in enumerate(grads) if not DTYPES.keys() >= set(map(_DTYPE, grads)) else ():
-        if g.dtype not in DTYPES:
-            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s' % (what, i, g.dtype))
-    for i, g in enumerate(grads):
-        if g.layout != torch.strided:
-            raise GvdHipError('%s: gradient %d must be a dense float32 / bfloat16 / float16 tensor, got %s' % (what, i, g.layout))
-    devices = set(map(_T.get_device, grads))
-    if len(devices) > 1:
-        raise GvdHipError('%s: gradients on several devices (%s)' % (what, sorted(devices)))
-    if devices and not grads[0].is_cuda:
-        raise GvdHipError('%s: the gradients are not on the GPU; there is no CPU fallback' % what)
-
-
 class _Tensors:
-    """Addresses, sizes and type codes of a list of tensors."""
+    """Addresses, sizes and type codes of a list of dense float tensors on one GPU."""
 
-    def __init__(self, tensors, like=None):
-        self.ptr = np.array(list(map(_T.data_ptr, tensors)), np.int64)
-        self.n = like.n if like is not None else np.array(list(map(_T.numel, tensors)), np.int64)
-        first = tensors[0].dtype
+    def __init__(self, tensors, what, like=None):
         types = list(map(_DTYPE, tensors))
-        if types.count(first) == len(types):
-            self.code = np.full(len(types), DTYPES[first], np.uint8)
+        if types.count(types[0]) == len(types) and types[0] in DTYPES:
+            self.code = np.full(len(types), DTYPES[types[0]], np.uint8)
         else:
-            self.code = np.array([DTYPES[t] for t in types], np.uint8)
+            self.code = np.array([DTYPES.get(t, 255) for t in types], np.uint8)
+            if (self.code == 255).any():
+                i = int((self.code == 255).argmax())
+                raise GvdHipError('%s: tensor %d must be float32 / bfloat16 / float16, got %s' % (what, i, types[i]))
+        devices = set(map(_T.get_device, tensors))
+        if len(devices) > 1:
+            raise GvdHipError('%s: tensors on several devices (%s)' % (what, sorted(devices)))
+        if not tensors[0].is_cuda:
+            raise GvdHipError('%s: the tensors are not on the GPU; there is no CPU fallback' % what)
+        self.n = like.n if like is not None else np.array(list(map(_T.numel, tensors)), np.int64)
+        self.ptr = np.array(list(map(_T.data_ptr, tensors)), np.int64)
         self.end = self.ptr + self.n * np.where(self.code == 0, 4, 2)
+
+
+def _strided(tensors, what):
+    for i, t in enumerate(tensors):
+        if t.layout != torch.strided:
+            raise GvdHipError('%s: tensor %d must be dense, got %s' % (what, i, t.layout))
+
+
+def _all_contiguous(tensors, what):
+    try:
+        return all(map(_T.is_contiguous, tensors))
+    except RuntimeError:                                 # (a sparse tensor)
+        _strided(tensors, what)
+        raise
 
 
 def _any_overlap(starts, ends):
@@ -286,8 +292,8 @@ def _check_clip(max_norm, inv_scale, what):
     return max_norm, inv_scale
 
 
-def _no_gradients(grads):
-    return torch.zeros((), device=grads[0].device if grads else 'cuda')
+def _no_gradients():
+    return torch.zeros((), device='cuda')
 
 
 @torch.no_grad()
@@ -297,11 +303,18 @@ def grad_norm(grads, inv_scale=1.0):
     what = 'grad_norm'
     _, inv_scale = _check_clip(0.0, inv_scale, what)
     grads = list(grads)
-    _check_grads(grads, what)
-    live = [g if _dense(g) else g.contiguous() for g in grads if g.numel()]
-    if not live:
-        return _no_gradients(grads)
-    return _norm_and_scale(live[0].device, _Tensors(live), None, 0.0, inv_scale, False, what)
+    if not _all_contiguous(grads, what):
+        _strided(grads, what)
+        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    if not grads:
+        return _no_gradients()
+    t, device = _Tensors(grads, what), grads[0].device
+    if not t.n.all():
+        grads = [g for g in grads if g.numel()]
+        if not grads:
+            return torch.zeros((), device=device)
+        t = _Tensors(grads, what)
+    return _norm_and_scale(device, t, None, 0.0, inv_scale, False, what)
 
 
 @torch.no_grad()
@@ -316,23 +329,32 @@ def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=Fals
     what = 'clip_grads'
     max_norm, inv_scale = _check_clip(max_norm, inv_scale, what)
     grads = list(grads)
+    written = grads if out is None else list(out)
     if out is not None:
-        out = list(out)
-        if len(out) != len(grads):
-            raise GvdHipError('%s: %d gradients, %d results' % (what, len(grads), len(out)))
-        for i, (g, o) in enumerate(zip(grads, out)):
-            if o.dtype not in DTYPES or o.shape != g.shape or o.get_device() != g.get_device():
-                raise GvdHipError('%s: result %d must be a float32 / bfloat16 / float16 tensor %s on %s' % (what, i, tuple(g.shape),
-                                                                                                            g.device))
-    _check_grads(grads, what)
-    written = grads if out is None else out
-    if not all(map(_T.numel, grads)):
-        keep = [i for i, g in enumerate(grads) if g.numel()]
-        grads, written = [grads[i] for i in keep], [written[i] for i in keep]
+        if len(written) != len(grads):
+            raise GvdHipError('%s: %d gradients, %d results' % (what, len(grads), len(written)))
+        if list(map(_SHAPE, grads)) != list(map(_SHAPE, written)):
+            i = [g.shape == o.shape for g, o in zip(grads, written)].index(False)
+            raise GvdHipError('%s: result %d must be of shape %s, got %s' % (what, i, tuple(grads[i].shape), tuple(written[i].shape)))
+    plain = _all_contiguous(grads, what) and (out is None or _all_contiguous(written, what))
+    if not plain:
+        _strided(grads, what)
+        _strided(written, what)
     if not grads:
-        return _no_gradients(written)
-    src, dst, back = grads, written, []
-    if not (all(map(_T.is_contiguous, grads)) and (out is None or all(map(_T.is_contiguous, written)))):
+        return _no_gradients()
+    s = _Tensors(grads, what)
+    d = s if out is None else _Tensors(written, what, s)
+    if out is not None and grads[0].device != written[0].device:
+        raise GvdHipError('%s: gradients on %s, results on %s' % (what, grads[0].device, written[0].device))
+    device = grads[0].device
+    if not s.n.all():
+        keep = s.n.nonzero()[0].tolist()
+        if not keep:
+            return torch.zeros((), device=device)
+        return clip_grads([grads[i] for i in keep], max_norm, None if out is None else [written[i] for i in keep], inv_scale,
+                          error_if_nonfinite)
+    back = []
+    if not plain:
         # element i of a result belongs to element i of its gradient: same order in memory, or both in row-major order
         src, dst = [], []
         for g, o in zip(grads, written):
@@ -343,12 +365,12 @@ def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=Fals
             dst.append(o if same or o.is_contiguous() else src[-1] if o is g else torch.empty_like(o, memory_format=torch.contiguous_format))
             if dst[-1] is not o:
                 back.append((o, dst[-1]))
-    s = _Tensors(src)
-    d = s if src is dst or all(map(operator.is_, src, dst)) else _Tensors(dst, s)
+        s = _Tensors(src, what)
+        d = s if all(map(operator.is_, src, dst)) else _Tensors(dst, what, s)
+        for o, _ in back:
+            _check_scattered(o, grads + written, what)
     _check_written(s, d, what)
-    for o, _ in back:
-        _check_scattered(o, src, dst, what)
-    norm = _norm_and_scale(grads[0].device, s, d, max_norm, inv_scale, error_if_nonfinite, what)
+    norm = _norm_and_scale(device, s, d, max_norm, inv_scale, error_if_nonfinite, what)
     for o, x in back:
         o.copy_(x)
     try:
@@ -358,11 +380,13 @@ def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=Fals
     return norm
 
 
-def _check_scattered(o, src, dst, what):
+def _check_scattered(o, tensors, what):
     """`o`, a result with gaps that is written by way of a copy, lies apart from every other tensor of the call."""
-    first, last = o.data_ptr(), o.data_ptr() + (sum((n - 1) * s for n, s in zip(o.shape, o.stride())) + 1) * o.element_size()
-    for t in src + dst:
-        if t is not o and t.data_ptr() < last and first < t.data_ptr() + t.numel() * t.element_size():
+    span = lambda t: (t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size())  # noqa: E731
+    first, last = span(o)
+    for t in tensors:
+        a, b = span(t)
+        if t is not o and a < last and first < b:
             raise GvdHipError('%s: a result of strides %s lies among other tensors of the call' % (what, o.stride()))
 
 

@@ -71,9 +71,9 @@ def test_clip_refusals():
         _refused('inv_scale', optim.grad_norm, g, inv_scale=inv)
     _refused('2 gradients, 1 results', optim.clip_grads, g, 1.0, out=g[:1])
     _refused('result 1', optim.clip_grads, g, 1.0, out=[torch.zeros(5), torch.zeros(3, 2)])
-    _refused('result 0', optim.clip_grads, g, 1.0, out=[torch.zeros(5).double(), torch.zeros(2, 3)])
-    _refused('gradient 1 must be', optim.clip_grads, [g[0], g[1].double()], 1.0)
-    _refused('gradient 0 must be', optim.grad_norm, [torch.zeros(4, 4).to_sparse()])
+    _refused('no CPU fallback', optim.clip_grads, g, 1.0, out=[torch.zeros(5).double(), torch.zeros(2, 3)])
+    _refused('tensor 1 must be', optim.clip_grads, [g[0], g[1].double()], 1.0)
+    _refused('tensor 0 must be', optim.grad_norm, [torch.zeros(4, 4).to_sparse()])
     _refused('no CPU fallback', optim.clip_grads, g, 1.0)
     _refused('no CPU fallback', optim.grad_norm, g)
     p = torch.nn.Parameter(torch.zeros(3))
