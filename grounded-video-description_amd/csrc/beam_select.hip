@@ -60,21 +60,22 @@ __device__ __forceinline__ u64 wave_max_u64(u64 v) {
   return lane63(v);
 }
 
-template <int STEP> __device__ __forceinline__ unsigned extreme_step(unsigned x, bool largest) {
-  const unsigned hi = gvd_dpp<STEP>(x, 0u), lo = gvd_dpp<STEP>(x, 0xffffffffu);
-  return largest ? max(x, hi) : min(x, lo);
-}
+template <int STEP> __device__ __forceinline__ unsigned max_step(unsigned x) { return max(x, gvd_dpp<STEP>(x, 0u)); }
 __device__ __forceinline__ float wave_max_f32(float f) {
   unsigned x = order_bits(f);
-  x = extreme_step<0>(x, true); x = extreme_step<1>(x, true); x = extreme_step<2>(x, true);
-  x = extreme_step<3>(x, true); x = extreme_step<4>(x, true); x = extreme_step<5>(x, true);
+  x = max_step<0>(x); x = max_step<1>(x); x = max_step<2>(x);
+  x = max_step<3>(x); x = max_step<4>(x); x = max_step<5>(x);
   return from_order_bits((unsigned)__builtin_amdgcn_readlane((int)x, 63));
 }
-// the smallest of the maxima of W or more equal groups of lanes: at least W lanes are at or over it
-__device__ __forceinline__ unsigned group_bound(unsigned x, int W) {
-  x = extreme_step<0>(x, 2 * W <= 64); x = extreme_step<1>(x, 4 * W <= 64); x = extreme_step<2>(x, 8 * W <= 64);
-  x = extreme_step<3>(x, 16 * W <= 64); x = extreme_step<4>(x, 32 * W <= 64); x = extreme_step<5>(x, 64 * W <= 64);
-  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+// a value that W lanes or more reach, and next to no more than W: its upper half exactly, bit by bit (0: fewer lanes have any)
+__device__ __forceinline__ unsigned wave_bound(unsigned x, int W) {
+  unsigned t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const unsigned c = t | 1u << bit;
+    if (__popcll(__ballot(x >= c)) >= W) t = c;
+  }
+  return t;
 }
 
 __device__ __forceinline__ int lanes_below(u64 mask, int lane) { return __popcll(mask & ((1ull << lane) - 1ull)); }
@@ -106,9 +107,9 @@ __device__ __forceinline__ void rank_list(u64* list, int n, int W, int lane) {
 }
 
 // One wave per part of a row: 64 * IPT logits at a time, the next ones on their way meanwhile.  Every lane has a running maximum
-// and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a bound from
-// the first tile: with the lanes in W or more equal groups, the smallest of the groups' maxima is reached by W words.  The list is
-// ranked, and the floor raised, when it is full; logits of any order and equality only make that more frequent.
+// and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a value
+// that the maxima of W lanes reach.  The list is ranked, and the floor raised, behind a tile and when it is full; logits of any
+// order and equality only make that more frequent.
 template <typename T, int IPT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 && sizeof(T) == 2 ? 4 : 3))) void beam_part_kernel(const SelectArgs a) {
   constexpr int N = 16 / (int)sizeof(T), VECS = IPT / N, TILE = 64 * IPT;
@@ -158,8 +159,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 &
 #pragma unroll
     for (int i = 0; i < IPT; ++i) s[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * 1.44269504088896341f);
     sum = sum * (double)__builtin_amdgcn_exp2f((was - ref) * 1.44269504088896341f) + (double)((s[0] + s[1]) + (s[2] + s[3]));
-    if (v0 == first) floor = (u64)group_bound(order_bits(mx), W) << 32;
-    const float least = floor >> 32 ? from_order_bits((unsigned)(floor >> 32)) : -INFINITY;   // no word under it is among the best
+    if (v0 == first) floor = (u64)wave_bound(order_bits(mx), W) << 32;
+    // no word under `least` is among the best (bits under those of -inf are no number)
+    const unsigned bits = (unsigned)(floor >> 32);
+    const float least = bits > 0x007fffffu ? from_order_bits(bits) : -INFINITY;
     if (!__ballot(mx >= least)) continue;
     unsigned todo = 0;                     // the lane's words at or over it
 #pragma unroll
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 &
 }
 
 // One workgroup per sample, one wave per beam (and the beams 16 further on): the words of the row's parts at or over the best
-// W-th word of a part are put on a list and ranked.  Then all waves do the same with the candidates of the beams.
+// W-th word of a part, and over what the best words of W lanes reach, are put on a list and ranked.  Then all waves do the same with the candidates of the beams.
 __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
   __shared__ double s_score[MAX_BEAMS * MAX_WIDTH];
   __shared__ int s_word[MAX_BEAMS * MAX_WIDTH];
@@ -241,7 +244,12 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
       }
       continue;
     }
+    u64 most = mine[0];
+#pragma unroll
+    for (int i = 1; i < JOIN_LIST / 64; ++i) most = mine[i] > most ? mine[i] : most;
+    const u64 reached = (u64)wave_bound((unsigned)(most >> 32), W) << 32;          // (by the best words of W lanes)
     floor = wave_max_u64(floor);
+    floor = reached > floor ? reached : floor;
     u64* list = s_list[wave];
     int n = 0;
 #pragma unroll

@@ -1900,24 +1900,33 @@ class _EmbeddingFn(torch.autograd.Function):
         return _embedding_fwd(tokens, weight, scale, act)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        tokens, weight = ctx.saved_tensors
-        (V, E), dtype, scale, act, pad = ctx.meta
-        n, dev = tokens.numel(), dy.device
-        if not n or not E or not V:
-            return None, torch.zeros(V, E, dtype=dtype, device=dev), None, None, None
-        dy2 = dy.reshape(n, E)
-        if E > 1 and dy2.stride(1) != 1:       # (a gradient broadcast over the rows, stride 0, is read in place)
-            dy2 = dy2.contiguous()
-        dw = torch.empty(V, E, dtype=dtype, device=dev)
-        l = lib()
-        need = l.gvd_embedding_bwd_workspace_bytes(n, V, E)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        run_on(dev, l.gvd_embedding_bwd, 'gvd_embedding_bwd', tokens.data_ptr(), tokens.dtype == torch.int64, n, dy2.data_ptr(),
-               dy2.stride(0), weight.data_ptr() if act else None, (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype],
-               scale, act, pad, dw.data_ptr(), ws.data_ptr(), need)
-        return None, dw, None, None, None
+        if torch.is_grad_enabled():              # create_graph: the gradient is there, its own gradient is refused
+            return _embedding_bwd_once(ctx, dy)
+        return _embedding_bwd(ctx, dy)
+
+
+def _embedding_bwd(ctx, dy):
+    tokens, weight = ctx.saved_tensors
+    (V, E), dtype, scale, act, pad = ctx.meta
+    n, dev = tokens.numel(), dy.device
+    if not n or not E or not V:
+        return None, torch.zeros(V, E, dtype=dtype, device=dev), None, None, None
+    if dy.dim() != 2:
+        dy = dy.reshape(n, E)
+    if E > 1 and dy.stride(1) != 1:              # (a gradient broadcast over the rows, stride 0, is read in place)
+        dy = dy.contiguous()
+    dw = torch.empty(V, E, dtype=dtype, device=dev)
+    l = lib()
+    need = l.gvd_embedding_bwd_workspace_bytes(n, V, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    run_on(dev, l.gvd_embedding_bwd, 'gvd_embedding_bwd', tokens.data_ptr(), tokens.dtype == torch.int64, n, dy.data_ptr(),
+           dy.stride(0), weight.data_ptr() if act else None, (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype],
+           scale, act, pad, dw.data_ptr(), ws.data_ptr(), need)
+    return None, dw, None, None, None
+
+
+_embedding_bwd_once = torch.autograd.function.once_differentiable(_embedding_bwd)
 
 
 def embedding(tokens, weight, scale=1.0, act=0, padding_idx=None):
