@@ -1912,6 +1912,8 @@ def _embedding_bwd(ctx, dy):
     n, dev = tokens.numel(), dy.device
     if not n or not E or not V:
         return None, torch.zeros(V, E, dtype=dtype, device=dev), None, None, None
+    if dy.dtype != dtype:
+        dy = dy.to(dtype)
     if dy.dim() != 2:
         dy = dy.reshape(n, E)
     if E > 1 and dy.stride(1) != 1:              # (a gradient broadcast over the rows, stride 0, is read in place)

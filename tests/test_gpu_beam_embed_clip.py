@@ -184,6 +184,24 @@ def test_embedding_gradient_against_differences():
             assert float(grad[v, e]) == float((up - down) / 0.5)
 
 
+def test_embedding_past_32_bits():
+    """A table, a result and a gradient of more than 2^32 bytes each (stores past the cache, nine tiles a sorting workgroup)."""
+    V, E, n = 1100003, 2048, 1050007
+    w = (torch.arange(V, device='cuda') % 61).to(torch.bfloat16).unsqueeze(1).expand(V, E).contiguous().requires_grad_()
+    tok = torch.arange(n, device='cuda') * 7 % V
+    tok[-5:] = V - 1
+    out = ops.embedding(tok, w, scale=2.0)
+    want = (tok % 61 * 2).to(torch.bfloat16)
+    assert torch.equal(out.detach()[:, ::1023], want.unsqueeze(1).expand(n, 3)) and torch.equal(out.detach()[-1], want[-1].expand(E))
+    dy = torch.randn(E, generator=gen(1), device='cuda').to(torch.bfloat16)
+    grad, = torch.autograd.grad(out, w, dy.expand(n, E))
+    times = torch.bincount(tok, minlength=V).float()
+    assert float(times.max()) < 8                               # (times * 2 * dy: exact in fp32, rounded once)
+    for cols in (slice(0, 3), slice(E - 2, E)):
+        assert torch.equal(grad[:, cols], (times.unsqueeze(1) * 2.0 * dy[cols].float()).to(torch.bfloat16))
+    assert torch.equal(grad[V - 1], (float(times[V - 1]) * 2.0 * dy.float()).to(torch.bfloat16))
+
+
 def test_embedding_refuses_a_second_derivative_and_sees_changed_tables():
     w = torch.randn(5, 4, device='cuda', requires_grad=True)
     tok = torch.zeros(3, dtype=torch.int64, device='cuda')
@@ -259,6 +277,20 @@ def test_clip_into_other_tensors(src, dst):
             gaps[at:at + s] = 7.0
             at += s + 1
         assert bool((gaps == 7.0).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=ids)
+def test_clip_more_than_the_cache_holds(dtype):
+    """Results of over 256 MB take the stores past the cache; in place and into views at odd offsets."""
+    sizes = [20000003, 8191, 60000001]
+    grads = make_grads(sizes, [dtype] * 3, 12)
+    flat = torch.zeros(sum(sizes) + 1, device='cuda')
+    out = list(torch.split(flat[1:], sizes))
+    norm = optim.clip_grads(grads, 100.0, out=out, inv_scale=0.5)
+    check_clip(grads, out, norm, 100.0, 0.5, 'apart')
+    was = [g.clone() for g in grads]
+    norm = optim.clip_grads(grads, 100.0)
+    check_clip(was, grads, norm, 100.0, 1.0, 'in place')
 
 
 def test_clip_strides():
@@ -378,9 +410,11 @@ def check_select(logits, scores, W=None, finished=None, eos=None, what=''):
     assert ((beam >= 0) & (beam < K)).all() and ((word >= 0) & (word < V)).all(), what
     rows = np.arange(B)[:, None]
     best, have = cand[rows, order], cand[rows, at]
-    # log-sum-exp: fp32 terms (2 u of the exponential, |x - max| u of its argument, weighted by the term: under log V + 1 in all) added
-    # 32 at a time in fp32; the score is rounded once
-    tol = (2 + 32 + math.log(V) + 1) * U[torch.float32]
+    # log-sum-exp: fp32 terms, each off by 2 u (the exponential, one unit in the last place) and by 2 |x - max| u (the difference
+    # and the product that make its argument); weighted by the terms, |x - max| is log V on average at most.  They are added 32
+    # at a time in fp32 (31 u), scaled from tile to tile and lane to lane (2 u and 2 |change of max| u, weighted likewise).  The
+    # score is rounded once.
+    tol = (2 + 31 + 2 + 4 * (math.log(V) + 1)) * U[torch.float32]
     fin = np.isfinite(best)
     assert (np.isfinite(sc.cpu().numpy()) == fin).all(), what
     assert (np.abs(sc.cpu().numpy()[fin].astype(np.float64) - have[fin]) <= tol + np.abs(have[fin]) * U[torch.float32]).all(), what
@@ -585,6 +619,42 @@ def test_other_streams():
     torch.cuda.synchronize()
     for e, bs, n in got:
         assert torch.equal(e, want_e) and torch.equal(n, want_n) and all(torch.equal(u, v) for u, v in zip(bs, want_b))
+
+
+def test_inference_mode_and_other_threads():
+    """Tensors without versions; two host threads at once, each on a stream of its own."""
+    import threading
+    with torch.inference_mode():
+        w = torch.randn(50, 16, generator=gen(1), device='cuda')
+        assert torch.equal(ops.embedding(torch.arange(50, device='cuda'), w), w)
+        g = torch.full((100,), 3.0, device='cuda')
+        optim.clip_grads([g], 3.0)
+        assert abs(float(g[0]) - 0.3) < 1e-6
+        x, s = beams(2, 3, 40, 5)
+        p = ops.beam_select(x, s)[1]
+        assert torch.equal(ops.reorder_rows([x], p)[0], x[p.view(-1)])
+    w = torch.randn(3000, 200, generator=gen(2), device='cuda')
+    tok = words('half', 20000, 3000, 3)
+    dy = torch.randn(20000, 200, generator=gen(4), device='cuda')
+    wl = w.detach().clone().requires_grad_()
+    want, = torch.autograd.grad(ops.embedding(tok, wl, act=1), wl, dy)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                v = wl.detach().clone().requires_grad_()
+                got, = torch.autograd.grad(ops.embedding(tok, v, act=1), v, dy)
+                if not torch.equal(got, want):
+                    bad.append(1)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_captured_and_replayed():
