@@ -4,7 +4,7 @@
 //   backward   dW[v,:]  = scale * act'(scale * W[v,:]) * sum over n with tok[n] = v, n ascending, of dy[n,:]
 //
 // (act' depends on the table row alone, so it multiplies the finished sum once.)  Both directions are bound by the rows they
-// move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable),
+// move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable; up to 4096 are listed by token instead),
 // every row of dW is summed by one owner in a fixed order and written once, rows without a token as zeros.  Sums are fp32.
 #include "dtypes.h"
 
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int
 }
 
 // ------------------------------------------------------------------------------------------- positions sorted by token
-// n <= RANK_MAX: the place of position i is the number of positions that go before it, counted directly: keys smaller, or
+// SMALL_MAX < n <= RANK_MAX: the place of position i is the number of positions that go before it, counted directly: keys smaller, or
 // equal and earlier.  n^2 comparisons (2 instructions each) spread over n / 64 workgroups of 16 waves.
 constexpr int RANK_MAX = 8192;
 constexpr int RANK_THREADS = 1024;
@@ -240,7 +240,6 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 // A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one wave
 // per group, so that no owner of a row adds up more than a few hundred rows whatever the tokens are.
 constexpr int GROUP = 32;
-constexpr int64_t LEVEL2_FROM = 4096;     // positions from which the second level pays for its launch
 
 struct SumArgs {
   const unsigned* skey; const unsigned* spos; int64_t n;
@@ -311,6 +310,120 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
     add_rows<float, N, 256>(a.part1 + (int64_t)g * GROUP * a.width, a.width, (unsigned)lane, GROUP, col, s);
   }
   if (col >= 0) gvd_store<float, N>((LEVEL == 1 ? a.part1 : a.part2) + (int64_t)g * a.width + col, s);
+}
+
+// ---------------------------------------------------------------------------------------------- few tokens: one launch
+// n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists the
+// positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than 32 positions are left for all
+// sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of a sort, groups and
+// rows: at these sizes a launch costs the host more than the work takes.
+constexpr int SMALL_MAX = 4096;
+constexpr int SMALL_ROWS = 64;
+constexpr int64_t SMALL_TABLE = 1 << 23;   // elements: two workgroups of SMALL_ROWS rows and 256 columns for every CU
+constexpr int SMALL_WAVES = 16;
+
+// row v = s, scaled
+template <typename T, int N>
+__device__ __forceinline__ void put_row(const SumArgs& a, int64_t v, int col, const float (&s)[N]) {
+  if (col < 0) return;
+  float x[N];
+  if (a.act) {
+    const typename GvdVec<T, N>::type w = fetch<T, N>(reinterpret_cast<const T*>(a.table) + v * a.ldt, col);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = (float)w[k] * a.scale > 0.f ? s[k] * a.scale : 0.f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = s[k] * a.scale;
+  }
+  gvd_store<T, N>(reinterpret_cast<T*>(a.dw) + v * a.width + col, x);
+}
+
+template <typename T, int N>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const SumArgs a, const void* tok, int tok64, int64_t pad, int rows) {
+  __shared__ unsigned s_list[SMALL_MAX];                     // row of the workgroup << 16 | position
+  __shared__ unsigned s_pos[SMALL_WAVES][128];
+  __shared__ float s_sum[SMALL_WAVES][64 * N];
+  __shared__ int s_count[SMALL_ROWS];
+  __shared__ int s_found[SMALL_WAVES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const unsigned unit = blockIdx.x / a.slices;
+  const int col = lane_column<N>(blockIdx.x - unit * a.slices, a.width);
+  const unsigned v0 = unit * (unsigned)rows, mine = a.vocab - v0 < (unsigned)rows ? a.vocab - v0 : (unsigned)rows;
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+  const int n = (int)a.n, each = (n + 64 * SMALL_WAVES - 1) / (64 * SMALL_WAVES) * 64;      // a wave looks at `each` tokens, 64 at a time
+  if (threadIdx.x < SMALL_ROWS) s_count[threadIdx.x] = 0;
+  unsigned row[SMALL_MAX / (64 * SMALL_WAVES)];
+#pragma unroll
+  for (int i = 0; i < SMALL_MAX / (64 * SMALL_WAVES); ++i) {
+    const int at = wave * each + 64 * i + lane;
+    row[i] = 64 * i < each && at < n ? token_key(tok, tok64, at, a.vocab, pad) - v0 : 0xffffffffu;
+  }
+  int found = 0;
+#pragma unroll
+  for (int i = 0; i < SMALL_MAX / (64 * SMALL_WAVES); ++i) found += __popcll(__ballot(row[i] < mine));
+  if (lane == 0) s_found[wave] = found;
+  __syncthreads();
+  int at = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < SMALL_WAVES; ++w) { at += w < wave ? s_found[w] : 0; total += s_found[w]; }
+#pragma unroll
+  for (int i = 0; i < SMALL_MAX / (64 * SMALL_WAVES); ++i) {
+    const unsigned long long in = __ballot(row[i] < mine);
+    if (row[i] < mine) {
+      s_list[at + __popcll(in & ((1ull << lane) - 1ull))] = row[i] << 16 | (unsigned)(wave * each + 64 * i + lane);
+      atomicAdd(&s_count[row[i]], 1);
+    }
+    at += __popcll(in);
+  }
+  __syncthreads();
+  // s += the positions of row r in list entries [from, to): collected first, so that 64 of them are added in one go
+  const auto add_listed = [&](unsigned r, int from, int to, float (&s)[N]) {
+    unsigned* pos = s_pos[wave];
+    int have = 0;
+    for (int i = from; i < to; i += 64) {
+      const unsigned e = i + lane < to ? s_list[i + lane] : 0xffffffffu;
+      const unsigned long long all = __ballot(e >> 16 == r);
+      if (e >> 16 == r) pos[have + __popcll(all & ((1ull << lane) - 1ull))] = e & 0xffffu;
+      have += __popcll(all);
+      if (have < 64 && i + 64 < to) continue;
+      wave_lds_fence();
+      const unsigned which = pos[lane], rest = pos[64 + lane];
+      wave_lds_fence();
+      pos[lane] = rest;
+      const int now = have < 64 ? have : 64;
+      add_rows<T, N, 256>(dy, a.ld, which, now, col, s);
+      have -= now;
+    }
+    wave_lds_fence();
+    if (have) add_rows<T, N, 256>(dy, a.ld, pos[lane], have, col, s);
+    wave_lds_fence();
+  };
+  for (unsigned r = wave; r < mine; r += SMALL_WAVES) {
+    if (s_count[r] > 32) continue;
+    float s[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = 0.f;
+    if (s_count[r]) add_listed(r, 0, total, s);
+    put_row<T, N>(a, v0 + r, col, s);
+  }
+  for (unsigned r = 0; r < mine; ++r) {
+    if (s_count[r] <= 32) continue;
+    float s[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = 0.f;
+    add_listed(r, total * wave / SMALL_WAVES, total * (wave + 1) / SMALL_WAVES, s);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s_sum[wave][k * 64 + lane] = s[k];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < SMALL_WAVES; ++w)
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k] += s_sum[w][k * 64 + lane];
+      put_row<T, N>(a, v0 + r, col, s);
+    }
+    __syncthreads();
+  }
 }
 
 // first sorted position i in [lo, n) with skey[i] >= v (RISE = 0), or skey[i] + i >= v (RISE = 1): 64 lanes look at 64 places at
@@ -398,7 +511,7 @@ __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
       const int64_t at = lane < head ? i + lane : g2 * GROUP + lane - head;
       add_rows<T, N, 128>(dy, a.ld, lane < ends ? a.spos[at] : 0, ends, col, s);
       const int64_t h1 = (g1 + GROUP - 1) / GROUP, h2 = g2 / GROUP;               // whole groups of groups
-      const bool two = a.n >= LEVEL2_FROM && h1 < h2;
+      const bool two = h1 < h2;
       for (int k = 0; k < 3; ++k) {              // groups before, groups of groups, groups behind them
         const int64_t from = k == 0 ? g1 : k == 1 ? h1 : two ? h2 * GROUP : g2, to = k == 0 ? (two ? h1 * GROUP : g2) : k == 1 ? (two ? h2 : h1) : g2;
         add_partials<N>(k == 1 ? a.part2 : a.part1, a.width, from, to, col, s);
@@ -447,13 +560,15 @@ int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 struct BwdSpace {
   int64_t skey, spos, key2, pos2, hist, part1, part2, bytes;
-  bool rank;
+  bool small, rank;
   int passes, bits, blocks;
   int64_t per;
 };
 
 BwdSpace bwd_space(int64_t n, int64_t vocab, int width) {
   BwdSpace s = {};
+  s.small = n <= SMALL_MAX && vocab * width <= SMALL_TABLE;
+  if (s.small) return s;                                // (no workspace)
   s.rank = n <= RANK_MAX;
   int bits = 1;
   while ((vocab >> bits) != 0) ++bits;                  // keys 0 ... vocab
@@ -497,6 +612,17 @@ int launch_fwd(const void* tok, int tok64, int64_t n, const void* table, int64_t
   return 0;
 }
 
+template <typename T, int N> int launch_small(SumArgs a, const void* tok, int tok64, int64_t pad, hipStream_t st) {
+  a.slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
+  int rows = 1;                            // rows a workgroup, up to 64, that still leave two workgroups to every CU
+  while (rows < SMALL_ROWS && (int64_t)a.vocab * a.slices > (int64_t)rows * 512) ++rows;
+  const int64_t groups = ((int64_t)a.vocab + rows - 1) / rows * a.slices;
+  if (groups > MAX_WAVES / SMALL_WAVES) return GVD_EINVAL;
+  hipLaunchKernelGGL((token_small_kernel<T, N>), dim3((unsigned)groups), dim3(64 * SMALL_WAVES), 0, st, a, tok, tok64, pad, rows);
+  GVD_CHECK_LAUNCH();
+  return 0;
+}
+
 template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
   a.slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
   const int64_t g1 = a.n / GROUP * a.slices, g2 = a.n / (GROUP * GROUP) * a.slices;
@@ -504,14 +630,10 @@ template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
   while (a.stretch < 64 && ((int64_t)a.vocab + a.n) / a.stretch * a.slices >= 2 * 4096) a.stretch *= 2;
   const int64_t owners = ((int64_t)a.vocab + a.n + a.stretch - 1) / a.stretch * a.slices;
   if (g1 > MAX_WAVES || owners > MAX_WAVES) return GVD_EINVAL;
-  if (a.n >= 64) {
-    hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
-    GVD_CHECK_LAUNCH();
-  }
-  if (a.n >= LEVEL2_FROM) {
-    hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
-    GVD_CHECK_LAUNCH();
-  }
+  hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
+  GVD_CHECK_LAUNCH();
+  hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
+  GVD_CHECK_LAUNCH();
   const bool past = (int64_t)a.vocab * a.width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
   hipLaunchKernelGGL((past ? token_rows_kernel<T, N, true> : token_rows_kernel<T, N, false>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
   GVD_CHECK_LAUNCH();
@@ -555,14 +677,27 @@ extern "C" size_t gvd_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, in
 extern "C" int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const void* dy, int64_t ld_dy, const void* table, int64_t ld,
                                  int64_t vocab, int width, int dtype, float scale, int act, int64_t padding_idx, void* dw,
                                  void* workspace, size_t workspace_bytes, gvd_stream_t stream) {
-  if (!tokens || !dy || !dw || !workspace || bad_shape(n, vocab, width, dtype) || ld_dy < 0 || (act && (!table || ld < width)))
+  if (!tokens || !dy || !dw || bad_shape(n, vocab, width, dtype) || ld_dy < 0 || (act && (!table || ld < width)))
     return GVD_EINVAL;
   const BwdSpace s = bwd_space(n, vocab, width);
-  if (workspace_bytes < (size_t)s.bytes || !gvd_aligned16(workspace)) return GVD_EINVAL;
+  if (s.bytes && (!workspace || workspace_bytes < (size_t)s.bytes || !gvd_aligned16(workspace))) return GVD_EINVAL;
   const hipStream_t st = gvd_s(stream);
   char* ws = reinterpret_cast<char*>(workspace);
   const auto at = [&](int64_t o) { return reinterpret_cast<unsigned*>(ws + o); };
   const int64_t pad = padding_idx < 0 ? -1 : padding_idx;
+  SumArgs a = {};
+  a.n = n;
+  a.dy = dy; a.ld = ld_dy;
+  a.table = table; a.ldt = ld;
+  a.dw = dw;
+  a.vocab = (unsigned)vocab; a.width = width; a.scale = scale; a.act = act;
+  if (s.small) {
+#define GVD_SMALL(T, N) launch_small<T, N>(a, tokens, tok64, pad, st)
+    GVD_BY_TYPE(GVD_SMALL)
+#undef GVD_SMALL
+  }
+  a.skey = at(s.skey); a.spos = at(s.spos);
+  a.part1 = reinterpret_cast<float*>(ws + s.part1); a.part2 = reinterpret_cast<float*>(ws + s.part2);
   if (s.rank) {
     hipLaunchKernelGGL(token_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(RANK_THREADS), 0, st, tokens, tok64, (int)n,
                        (unsigned)vocab, pad, at(s.skey), at(s.spos));
@@ -583,13 +718,6 @@ extern "C" int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const
       GVD_CHECK_LAUNCH();
     }
   }
-  SumArgs a = {};
-  a.skey = at(s.skey); a.spos = at(s.spos); a.n = n;
-  a.dy = dy; a.ld = ld_dy;
-  a.part1 = reinterpret_cast<float*>(ws + s.part1); a.part2 = reinterpret_cast<float*>(ws + s.part2);
-  a.table = table; a.ldt = ld;
-  a.dw = dw;
-  a.vocab = (unsigned)vocab; a.width = width; a.scale = scale; a.act = act;
 #define GVD_SUMS(T, N) launch_sums<T, N>(a, st)
   GVD_BY_TYPE(GVD_SUMS)
 #undef GVD_SUMS

@@ -1921,10 +1921,10 @@ def _embedding_bwd(ctx, dy):
     dw = torch.empty(V, E, dtype=dtype, device=dev)
     l = lib()
     need = l.gvd_embedding_bwd_workspace_bytes(n, V, E)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     run_on(dev, l.gvd_embedding_bwd, 'gvd_embedding_bwd', tokens.data_ptr(), tokens.dtype == torch.int64, n, dy.data_ptr(),
            dy.stride(0), weight.data_ptr() if act else None, (weight.stride(0) if V > 1 else E) if act else 0, V, E, DTYPES[dtype],
-           scale, act, pad, dw.data_ptr(), ws.data_ptr(), need)
+           scale, act, pad, dw.data_ptr(), ws.data_ptr() if need else None, need)
     return None, dw, None, None, None
 
 

@@ -125,12 +125,12 @@ def test_c_entries_refuse_before_they_launch():
     assert l.gvd_embedding_fwd(a, 1, 0, a, 8, 10, 8, 0, 1.0, 0, a, 8, None) == -1
     assert l.gvd_embedding_fwd(None, 1, 4, a, 8, 10, 8, 0, 1.0, 0, a, 8, None) == -1
     assert l.gvd_embedding_fwd(a, 1, (1 << 25) + 1, a, 8, 10, 8, 0, 1.0, 0, a, 8, None) == -1
-    need = l.gvd_embedding_bwd_workspace_bytes(1000, 50, 8)
-    assert need > 0 and l.gvd_embedding_bwd_workspace_bytes(0, 50, 8) == 0
-    assert l.gvd_embedding_bwd(a, 1, 1000, a, 8, a, 8, 50, 8, 0, 1.0, 0, -1, a, a, need - 1, None) == -1
-    assert l.gvd_embedding_bwd(a, 1, 1000, a, 8, None, 8, 50, 8, 0, 1.0, 1, -1, a, a, need, None) == -1    # act without its table
-    assert l.gvd_embedding_bwd(a, 1, 1000, a, -8, a, 8, 50, 8, 0, 1.0, 0, -1, a, a, need, None) == -1
-    assert l.gvd_embedding_bwd(a, 1, 1000, a, 8, a, 8, 50, 8, 0, 1.0, 0, -1, a, C.c_void_p(4100), need, None) == -1
+    need = l.gvd_embedding_bwd_workspace_bytes(5000, 50, 8)
+    assert need > 0 and l.gvd_embedding_bwd_workspace_bytes(1000, 50, 8) == 0 and l.gvd_embedding_bwd_workspace_bytes(0, 50, 8) == 0
+    assert l.gvd_embedding_bwd(a, 1, 5000, a, 8, a, 8, 50, 8, 0, 1.0, 0, -1, a, a, need - 1, None) == -1
+    assert l.gvd_embedding_bwd(a, 1, 5000, a, 8, None, 8, 50, 8, 0, 1.0, 1, -1, a, a, need, None) == -1    # act without its table
+    assert l.gvd_embedding_bwd(a, 1, 5000, a, -8, a, 8, 50, 8, 0, 1.0, 0, -1, a, a, need, None) == -1
+    assert l.gvd_embedding_bwd(a, 1, 5000, a, 8, a, 8, 50, 8, 0, 1.0, 0, -1, a, C.c_void_p(4100), need, None) == -1
 
     g = hip.GradGroup()
     c = hip.GradClip(1.0, 1.0)

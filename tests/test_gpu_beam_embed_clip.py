@@ -98,7 +98,7 @@ def test_embedding_sizes(n, V, E, dtype):
 
 
 @pytest.mark.parametrize('kind', ['one', 'half', 'skew', 'down'])
-@pytest.mark.parametrize('n,V,E', [(1280, 5000, 64), (3000, 17, 24), (20000, 5000, 96), (150001, 70000, 16), (140000, 400, 8)])
+@pytest.mark.parametrize('n,V,E', [(1280, 5000, 64), (3000, 17, 24), (4096, 900, 130), (4097, 900, 130), (7000, 40, 70), (20000, 5000, 96), (150001, 70000, 16), (140000, 400, 8)])
 def test_embedding_repeated_tokens(kind, n, V, E):
     """Tokens that fill whole groups of 64 and of 4096 sorted positions, every sort path; int32 tokens; the same bits twice."""
     tok = words(kind, n, V, n, torch.int32)
