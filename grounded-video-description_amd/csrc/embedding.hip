@@ -32,7 +32,9 @@ template <int N> __device__ __forceinline__ int lane_column(unsigned slice, int 
 
 // ------------------------------------------------------------------------------------------------------------- forward
 // One wave per R rows and 64 * N columns (a slice); the R tokens, then the R rows, are on their way together.  Waves next to each
-// other take the slices of the same rows, so that a row is one stretch of memory traffic.
+// other take the slices of the same rows, so that a row is one stretch of memory traffic.  Bound by the rows: 131072 x 2048
+// bf16 take 121 us (5.5 TB/s of rows read once and written) with stores past the cache, 146 us without; R = 2 and 8 take 132.
+// One decode step (5 x 512 fp32): 1.8 us, the launch.
 template <typename T, int N, int R, bool PAST>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int tok64, int64_t n, const T* __restrict__ table,
                                                             int64_t ld, unsigned vocab, int width, float scale, int act,
@@ -69,8 +71,9 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int
 }
 
 // ------------------------------------------------------------------------------------------- positions sorted by token
-// SMALL_MAX < n <= RANK_MAX: the place of position i is the number of positions that go before it, counted directly: keys smaller, or
-// equal and earlier.  n^2 comparisons (2 instructions each) spread over n / 64 workgroups of 16 waves.
+// n <= RANK_MAX: the place of position i is the number of positions that go before it, counted directly: keys smaller, or
+// equal and earlier.  n^2 comparisons (2 instructions each) spread over n / 64 workgroups of 16 waves: 6.5 us for 2049 positions
+// where the two launches of a counting sort's one pass take 11.
 constexpr int RANK_MAX = 8192;
 constexpr int RANK_THREADS = 1024;
 
@@ -113,7 +116,8 @@ __global__ __launch_bounds__(RANK_THREADS) void token_rank_kernel(const void* to
 
 // Larger n: stable counting sorts by digits of up to 9 bits, least significant first.  The positions are cut into at most
 // SORT_BLOCKS contiguous parts, one workgroup each: a launch counts every part's digits, the next one places them, each
-// workgroup adding up the counts before its own by itself.  A wave takes 64 consecutive positions at a time; lanes of equal digit
+// workgroup adding up the counts before its own by itself (32768 positions: 3.5 + 7.6 us a pass; 131072: 4.8 + 11.1.  Counting the
+// next pass's digits by atomics while placing took as long as the launch it saves).  A wave takes 64 consecutive positions at a time; lanes of equal digit
 // find each other by ballots, so equal digits keep their order.
 constexpr int SORT_BLOCKS = 128;
 constexpr int SORT_BITS = 9;
@@ -238,7 +242,8 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 
 // ------------------------------------------------------------------------------------------------------- sums by token
 // A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one wave
-// per group, so that no owner of a row adds up more than a few hundred rows whatever the tokens are.
+// per group with 16 rows on their way, so that no owner of a row adds up more than a few hundred rows whatever the tokens are
+// (131072 positions of 2048 bf16, half of them in such tokens: 50 us, 5.2 TB/s).
 constexpr int GROUP = 32;
 
 struct SumArgs {
@@ -316,7 +321,9 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
 // n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists the
 // positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than 32 positions are left for all
 // sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of a sort, groups and
-// rows: at these sizes a launch costs the host more than the work takes.
+// rows: at these sizes a launch costs the host (4 us) as much as the work takes.  1280 words, 5000 x 512 fp32: 19 us where the three
+// launches took 18 and 8 us more of the host; 2049 words, 432 x 301 fp16: 12 us, and 21.  Above SMALL_TABLE the workgroups no
+// longer run side by side, and the looking at all tokens shows: 4096 words, 50000 x 1024 bf16 took 54 us, sorted 31.
 constexpr int SMALL_MAX = 4096;
 constexpr int SMALL_ROWS = 64;
 constexpr int64_t SMALL_TABLE = 1 << 23;   // elements: two workgroups of SMALL_ROWS rows and 256 columns for every CU
@@ -448,8 +455,10 @@ __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_
 // The rows of the table, each followed by its sorted positions, are one sequence of vocab + n entries: row v is entry
 // v + (positions of smaller keys).  It is cut into stretches of `stretch` entries, and a wave owns the rows that lie in its
 // stretch (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows
-// without a position as zeros.  So no wave has much more to do than another, whatever the tokens are.  It walks 64 sorted
-// positions at a time; the dy rows of several tokens are on their way together.
+// without a position as zeros.  So no wave has much more to do than another, whatever the tokens are (equal numbers of rows a wave
+// took 394 us instead of 33 for 32768 words of falling frequency: the frequent ones lie side by side).  It walks 64 sorted
+// positions at a time; the dy rows of several tokens are on their way together.  Bound by dy and dw: 131072 x 2048 bf16 of
+// each, 176 us, 4.6 TB/s of what is left of dy and dw.
 template <typename T, int N, bool PAST>
 __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
   const unsigned id = wave_id(), unit = id / a.slices;
@@ -630,10 +639,14 @@ template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
   while (a.stretch < 64 && ((int64_t)a.vocab + a.n) / a.stretch * a.slices >= 2 * 4096) a.stretch *= 2;
   const int64_t owners = ((int64_t)a.vocab + a.n + a.stretch - 1) / a.stretch * a.slices;
   if (g1 > MAX_WAVES || owners > MAX_WAVES) return GVD_EINVAL;
-  hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
-  GVD_CHECK_LAUNCH();
-  hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
-  GVD_CHECK_LAUNCH();
+  if (a.n >= 64) {
+    hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
+    GVD_CHECK_LAUNCH();
+  }
+  if (g2) {
+    hipLaunchKernelGGL((token_group_kernel<T, N, 2>), dim3((unsigned)((g2 + 3) / 4)), dim3(256), 0, st, a);
+    GVD_CHECK_LAUNCH();
+  }
   const bool past = (int64_t)a.vocab * a.width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
   hipLaunchKernelGGL((past ? token_rows_kernel<T, N, true> : token_rows_kernel<T, N, false>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
   GVD_CHECK_LAUNCH();

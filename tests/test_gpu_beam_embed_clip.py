@@ -108,6 +108,16 @@ def test_embedding_repeated_tokens(kind, n, V, E):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize('kind', ['uniform', 'one', 'half'])
+@pytest.mark.parametrize('n', [1, 5, 31, 63, 64, 65, 1000, 1023, 1024, 1025, 4096])
+def test_embedding_few_tokens_of_a_big_table(n, kind):
+    """Tables that are sorted for, however few the tokens."""
+    V, E = 70001, 129
+    tok = words(kind, n, V, n)
+    w = torch.randn(V, E, generator=gen(3), device='cuda')
+    check_embedding(tok, w, 1.5, 1, what='%s %d' % (kind, n))
+
+
 @pytest.mark.parametrize('n', [100, 9000])
 def test_embedding_tokens_outside_and_padding(n):
     V, E = 37, 20
