@@ -72,8 +72,8 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int
 
 // ------------------------------------------------------------------------------------------- positions sorted by token
 // n <= RANK_MAX: the place of position i is the number of positions that go before it, counted directly: keys smaller, or
-// equal and earlier.  n^2 comparisons (2 instructions each) spread over n / 64 workgroups of 16 waves: 6.5 us for 2049 positions
-// where the two launches of a counting sort's one pass take 11.
+// equal and earlier.  n^2 comparisons (2 instructions each) spread over n / 64 workgroups of 16 waves.  The whole backward with
+// it and with the counting sort, us with events: 8192 words, 5000 x 512 fp32, 38 and 44.5; 16384, 50000 x 512 bf16, 57 and 53.
 constexpr int RANK_MAX = 8192;
 constexpr int RANK_THREADS = 1024;
 
@@ -319,15 +319,17 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
 
 // ---------------------------------------------------------------------------------------------- few tokens: one launch
 // n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists the
-// positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than 32 positions are left for all
+// positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than SMALL_ALONE positions are left for all
 // sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of a sort, groups and
-// rows: at these sizes a launch costs the host (4 us) as much as the work takes.  1280 words, 5000 x 512 fp32: 19 us where the three
-// launches took 18 and 8 us more of the host; 2049 words, 432 x 301 fp16: 12 us, and 21.  Above SMALL_TABLE the workgroups no
-// longer run side by side, and the looking at all tokens shows: 4096 words, 50000 x 1024 bf16 took 54 us, sorted 31.
+// rows: at these sizes a launch costs the host (4 us) as much as the work takes.  Measured with events (some 5 us of them the
+// events'), words of falling frequency, against the three launches: 1280 words, 5000 x 512 fp32, 16.8 and 20.7 us; 2049 words, 432 x
+// 301 fp16, 16.6 and 26.0; 4096 words, 5000 x 512 fp32, 31.5 and 28.6, and 8 us less of the host.  Above SMALL_TABLE the
+// workgroups no longer run side by side, and the looking at all tokens shows: 256 words, 50000 x 1024 bf16, 48.3 and 27.4 us.
 constexpr int SMALL_MAX = 4096;
 constexpr int SMALL_ROWS = 64;
 constexpr int64_t SMALL_TABLE = 1 << 23;   // elements: two workgroups of SMALL_ROWS rows and 256 columns for every CU
 constexpr int SMALL_WAVES = 16;
+constexpr int SMALL_ALONE = 128;            // positions that a wave adds up by itself: eight times 16 on their way
 
 // row v = s, scaled
 template <typename T, int N>
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const Sum
     wave_lds_fence();
   };
   for (unsigned r = wave; r < mine; r += SMALL_WAVES) {
-    if (s_count[r] > 32) continue;
+    if (s_count[r] > SMALL_ALONE) continue;
     float s[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = 0.f;
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const Sum
     put_row<T, N>(a, v0 + r, col, s);
   }
   for (unsigned r = 0; r < mine; ++r) {
-    if (s_count[r] <= 32) continue;
+    if (s_count[r] <= SMALL_ALONE) continue;
     float s[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = 0.f;
@@ -623,8 +625,11 @@ int launch_fwd(const void* tok, int tok64, int64_t n, const void* table, int64_t
 
 template <typename T, int N> int launch_small(SumArgs a, const void* tok, int tok64, int64_t pad, hipStream_t st) {
   a.slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
-  int rows = 1;                            // rows a workgroup, up to 64, that still leave two workgroups to every CU
-  while (rows < SMALL_ROWS && (int64_t)a.vocab * a.slices > (int64_t)rows * 512) ++rows;
+  // rows a workgroup, up to 64, for two workgroups to every CU, or four: fewer frequent words in one workgroup, but all tokens
+  // looked at twice as often (5000 x 512 fp32, us with events: 5 words 11.1 and 14.3, 1280 18.6 and 16.8, 4096 39 and 31.5)
+  const int64_t groups_wanted = a.n <= 512 ? 512 : 1024;
+  int rows = 1;
+  while (rows < SMALL_ROWS && (int64_t)a.vocab * a.slices > rows * groups_wanted) ++rows;
   const int64_t groups = ((int64_t)a.vocab + rows - 1) / rows * a.slices;
   if (groups > MAX_WAVES / SMALL_WAVES) return GVD_EINVAL;
   hipLaunchKernelGGL((token_small_kernel<T, N>), dim3((unsigned)groups), dim3(64 * SMALL_WAVES), 0, st, a, tok, tok64, pad, rows);
