@@ -245,6 +245,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 // per group with 16 rows on their way, so that no owner of a row adds up more than a few hundred rows whatever the tokens are
 // (131072 positions of 2048 bf16, half of them in such tokens: 50 us, 5.2 TB/s).
 constexpr int GROUP = 32;
+constexpr int STRETCH = 32;               // 8, 16 and 32 take the same time, 64 up to a fifth more
 
 struct SumArgs {
   const unsigned* skey; const unsigned* spos; int64_t n;
@@ -253,7 +254,7 @@ struct SumArgs {
   const void* table; int64_t ldt;         // for act'
   void* dw;
   unsigned vocab; int width; float scale; int act;
-  unsigned slices; int stretch;
+  unsigned slices;
 };
 
 // a lane's N columns of a row, as loaded (rows in flight cost half the registers in 16-bit types)
@@ -455,7 +456,7 @@ __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_
 }
 
 // The rows of the table, each followed by its sorted positions, are one sequence of vocab + n entries: row v is entry
-// v + (positions of smaller keys).  It is cut into stretches of `stretch` entries, and a wave owns the rows that lie in its
+// v + (positions of smaller keys).  It is cut into stretches of STRETCH entries, and a wave owns the rows that lie in its
 // stretch (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows
 // without a position as zeros.  So no wave has much more to do than another, whatever the tokens are (equal numbers of rows a wave
 // took 394 us instead of 33 for 32768 words of falling frequency: the frequent ones lie side by side).  It walks 64 sorted
@@ -465,7 +466,7 @@ template <typename T, int N, bool PAST>
 __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
   const unsigned id = wave_id(), unit = id / a.slices;
   const int lane = threadIdx.x & 63;
-  const int64_t d0 = (int64_t)unit * a.stretch, d1 = d0 + a.stretch;
+  const int64_t d0 = (int64_t)unit * STRETCH, d1 = d0 + STRETCH;
   if (d0 >= (int64_t)a.vocab + a.n) return;
   const int col = lane_column<N>(id - unit * a.slices, a.width);
   const T* dy = reinterpret_cast<const T*>(a.dy);
@@ -640,9 +641,7 @@ template <typename T, int N> int launch_small(SumArgs a, const void* tok, int to
 template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
   a.slices = (unsigned)((a.width + 64 * N - 1) / (64 * N));
   const int64_t g1 = a.n / GROUP * a.slices, g2 = a.n / (GROUP * GROUP) * a.slices;
-  a.stretch = 8;                           // entries a wave, up to 64, that still leave four waves to every SIMD
-  while (a.stretch < 64 && ((int64_t)a.vocab + a.n) / a.stretch * a.slices >= 2 * 4096) a.stretch *= 2;
-  const int64_t owners = ((int64_t)a.vocab + a.n + a.stretch - 1) / a.stretch * a.slices;
+  const int64_t owners = ((int64_t)a.vocab + a.n + STRETCH - 1) / STRETCH * a.slices;
   if (g1 > MAX_WAVES || owners > MAX_WAVES) return GVD_EINVAL;
   if (a.n >= 64) {
     hipLaunchKernelGGL((token_group_kernel<T, N, 1>), dim3((unsigned)((g1 + 3) / 4)), dim3(256), 0, st, a);
