@@ -52,7 +52,8 @@ template <int STEP> __device__ __forceinline__ u64 max_step(u64 x) {
   return o > x ? o : x;
 }
 __device__ __forceinline__ u64 lane63(u64 x) {
-  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, 63) | (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), 63) << 32;
+  const u64 hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), 63);
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, 63) | hi << 32;
 }
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
   v = max_step<0>(v); v = max_step<1>(v); v = max_step<2>(v);
@@ -106,16 +107,17 @@ __device__ __forceinline__ void rank_list(u64* list, int n, int W, int lane) {
   wave_lds_fence();
 }
 
-// One wave per part of a row: 64 * IPT logits at a time, the next ones on their way meanwhile.  Every lane has a running maximum
-// and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a value
-// that the maxima of W lanes reach.  The list is ranked, and the floor raised, behind a tile and when it is full; logits of any
-// order and equality only make that more frequent.  A wave works by itself, without a barrier: 256 rows of 131072 bf16 logits take
-// 29 us (the hits of the list are 6 of them, the exponentials none: loads and latency bound it), 256 rows fp32 30 us (4.0 TB/s),
-// 5 rows of 5000 fp32 4.3 us.  The same with a workgroup per part, barriers and a list of its own: 66 us.  Code is kept small (a lane
-// finds its next word by selecting, not by 32 copies of the append): at one tile a wave, fetching 50 KB of instructions was most
-// of the time.
+// One wave per part of a row: 64 * IPT logits at a time, the next ones on their way meanwhile.  Every lane has a running
+// maximum and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a
+// value that the maxima of W lanes reach.  The list is ranked, and the floor raised, behind a tile and when it is full; logits
+// of any order and equality only make that more frequent.  A wave works by itself, without a barrier: 256 rows of 131072 bf16
+// logits take 29 us (the hits of the list are 6 of them, the exponentials none: loads and latency bound it), 256 rows fp32 30
+// us (4.0 TB/s), 5 rows of 5000 fp32 4.3 us.  The same with a workgroup per part, barriers and a list of its own: 66 us.  Code
+// is kept small (a lane finds its next word by selecting, not by 32 copies of the append): at one tile a wave, fetching 50 KB
+// of instructions was most of the time.
 template <typename T, int IPT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 && sizeof(T) == 2 ? 4 : 3))) void beam_part_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 && sizeof(T) == 2 ? 4 : 3)))
+void beam_part_kernel(const SelectArgs a) {
   constexpr int N = 16 / (int)sizeof(T), VECS = IPT / N, TILE = 64 * IPT;
   typedef typename GvdVec<T, N>::type Vec;
   typedef typename GvdVec<T, N>::loose Loose;
@@ -202,8 +204,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 &
 }
 
 // One workgroup per sample, one wave per beam (and the beams 16 further on): the words of the row's parts at or over the best
-// W-th word of a part, and over what the best words of W lanes reach, are put on a list and ranked.  Then all waves do the same with the candidates of the beams.  A chain of
-// dependent steps: 5 us for 5 beams, 10 us for 15 samples of 12 beams (23 us when every listed word was ranked against every other).
+// W-th word of a part, and over what the best words of W lanes reach, are put on a list and ranked.  Then all waves do the same
+// with the candidates of the beams.  A chain of dependent steps: 5 us for 5 beams, 10 us for 15 samples of 12 beams (23 us when
+// every listed word was ranked against every other).
 __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
   __shared__ double s_score[MAX_BEAMS * MAX_WIDTH];
   __shared__ int s_word[MAX_BEAMS * MAX_WIDTH];
@@ -342,8 +345,9 @@ bool bad_select_shape(int B, int K, int V, int W) {
 
 // ------------------------------------------------------------------------------------------------------------- reorder
 // dst[o, r, :] = src[o, index[r], :], up to GVD_REORDER_MAX_TENSORS tensors in a launch.  A copy: bound by reading and writing
-// the rows once (2 caches of 256 x 1 MB: 129 us, 8.3 TB/s of rows read and written: parents repeat, and come from the cache).  A thread copies four units of 16 bytes; the last unit of a row is moved back so that it ends with the row
-// (rows under 16 bytes: units of 8, 4 or 1 bytes).
+// the rows once (2 caches of 256 x 1 MB: 129 us, 8.3 TB/s of rows read and written: parents repeat, and come from the cache).
+// A thread copies four units of 16 bytes; the last unit of a row is moved back so that it ends with the row (rows under 16
+// bytes: units of 8, 4 or 1 bytes).
 constexpr int UNITS = 1024;               // units of one workgroup
 
 template <int BYTES> struct Unit;

@@ -53,9 +53,9 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Reductions over a wave on the vector ALU: a lane takes its partner's value by DPP - within 4, 8, 16 lanes, then lane 15 of a row of
-// 16 to the next row, lane 31 to the upper half - so that lane 63 ends with the result (a shuffle goes by way of the LDS unit and
-// takes some ten times as long).  `none`: what lanes without a partner take.
+// Reductions over a wave on the vector ALU: a lane takes its partner's value by DPP - within 4, 8, 16 lanes, then lane 15 of a
+// row of 16 to the next row, lane 31 to the upper half - so that lane 63 ends with the result (a shuffle goes by way of the LDS
+// unit and takes some ten times as long).  `none`: what lanes without a partner take.
 template <int STEP> __device__ __forceinline__ unsigned gvd_dpp(unsigned x, unsigned none) {
   constexpr int ctrl[6] = {0xb1, 0x4e, 0x141, 0x140, 0x142, 0x143};      // quad 1032, quad 2301, half row and row mirrored, broadcasts
   constexpr int rows[6] = {0xf, 0xf, 0xf, 0xf, 0xa, 0xc};

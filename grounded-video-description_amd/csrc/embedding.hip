@@ -4,8 +4,9 @@
 //   backward   dW[v,:]  = scale * act'(scale * W[v,:]) * sum over n with tok[n] = v, n ascending, of dy[n,:]
 //
 // (act' depends on the table row alone, so it multiplies the finished sum once.)  Both directions are bound by the rows they
-// move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable; up to 4096 are listed by token instead),
-// every row of dW is summed by one owner in a fixed order and written once, rows without a token as zeros.  Sums are fp32.
+// move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable;
+// up to 4096 are listed by token instead), every row of dW is summed by one owner in a fixed order and written once, rows
+// without a token as zeros.  Sums are fp32.
 #include "dtypes.h"
 
 namespace {
@@ -22,19 +23,19 @@ __device__ __forceinline__ unsigned wave_id() {
   return __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));          // (workgroups of four waves)
 }
 
-// A lane's first column in slice `slice` of 64 * N columns; -1: none.  The last lane of a row is moved back so that it ends with the
-// row: it does some of its neighbour's columns again, the same sums in the same order, instead of a part of a vector (host: the
-// width is N at least).
+// A lane's first column in slice `slice` of 64 * N columns; -1: none.  The last lane of a row is moved back so that it ends
+// with the row: it does some of its neighbour's columns again, the same sums in the same order, instead of a part of a vector
+// (host: the width is N at least).
 template <int N> __device__ __forceinline__ int lane_column(unsigned slice, int width) {
   const int col = (int)(slice * 64 + (threadIdx.x & 63)) * N;
   return col >= width ? -1 : col <= width - N ? col : width - N;
 }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-// One wave per R rows and 64 * N columns (a slice); the R tokens, then the R rows, are on their way together.  Waves next to each
-// other take the slices of the same rows, so that a row is one stretch of memory traffic.  Bound by the rows: 131072 x 2048
-// bf16 take 121 us (5.5 TB/s of rows read once and written) with stores past the cache, 146 us without; R = 2 and 8 take 132.
-// One decode step (5 x 512 fp32): 1.8 us, the launch.
+// One wave per R rows and 64 * N columns (a slice); the R tokens, then the R rows, are on their way together.  Waves next to
+// each other take the slices of the same rows, so that a row is one stretch of memory traffic.  Bound by the rows: 131072 x
+// 2048 bf16 take 121 us (5.5 TB/s of rows read once and written) with stores past the cache, 146 us without; R = 2 and 8 take
+// 132. One decode step (5 x 512 fp32): 1.8 us, the launch.
 template <typename T, int N, int R, bool PAST>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* tok, int tok64, int64_t n, const T* __restrict__ table,
                                                             int64_t ld, unsigned vocab, int width, float scale, int act,
@@ -116,9 +117,9 @@ __global__ __launch_bounds__(RANK_THREADS) void token_rank_kernel(const void* to
 
 // Larger n: stable counting sorts by digits of up to 9 bits, least significant first.  The positions are cut into at most
 // SORT_BLOCKS contiguous parts, one workgroup each: a launch counts every part's digits, the next one places them, each
-// workgroup adding up the counts before its own by itself (32768 positions: 3.5 + 7.6 us a pass; 131072: 4.8 + 11.1.  Counting the
-// next pass's digits by atomics while placing took as long as the launch it saves).  A wave takes 64 consecutive positions at a time; lanes of equal digit
-// find each other by ballots, so equal digits keep their order.
+// workgroup adding up the counts before its own by itself (32768 positions: 3.5 + 7.6 us a pass; 131072: 4.8 + 11.1.  Counting
+// the next pass's digits by atomics while placing took as long as the launch it saves).  A wave takes 64 consecutive positions
+// at a time; lanes of equal digit find each other by ballots, so equal digits keep their order.
 constexpr int SORT_BLOCKS = 128;
 constexpr int SORT_BITS = 9;
 constexpr int SORT_DIGITS = 1 << SORT_BITS;
@@ -241,9 +242,9 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 }
 
 // ------------------------------------------------------------------------------------------------------- sums by token
-// A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one wave
-// per group with 16 rows on their way, so that no owner of a row adds up more than a few hundred rows whatever the tokens are
-// (131072 positions of 2048 bf16, half of them in such tokens: 50 us, 5.2 TB/s).
+// A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one
+// wave per group with 16 rows on their way, so that no owner of a row adds up more than a few hundred rows whatever the tokens
+// are (131072 positions of 2048 bf16, half of them in such tokens: 50 us, 5.2 TB/s).
 constexpr int GROUP = 32;
 constexpr int STRETCH = 32;               // 8, 16 and 32 take the same time, 64 up to a fifth more
 
@@ -263,8 +264,8 @@ template <typename T, int N> __device__ __forceinline__ typename GvdVec<T, N>::t
   return *reinterpret_cast<const typename GvdVec<T, N>::loose*>(row + col);
 }
 
-// s += `count` (<= 64) rows of x, in order: row i is the one that lane i names (`which`); FLIGHT bytes of a lane on their way at
-// a time, 16 rows at most
+// s += `count` (<= 64) rows of x, in order: row i is the one that lane i names (`which`); FLIGHT bytes of a lane on their way
+// at a time, 16 rows at most
 template <typename T, int N, int FLIGHT>
 __device__ __forceinline__ void add_rows(const T* x, int64_t ld, unsigned which, int count, int col, float (&s)[N]) {
   constexpr int BATCH = FLIGHT / (int)(sizeof(T) * N) < 16 ? FLIGHT / (int)(sizeof(T) * N) : 16;
@@ -319,13 +320,14 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- few tokens: one launch
-// n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists the
-// positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than SMALL_ALONE positions are left for all
-// sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of a sort, groups and
-// rows: at these sizes a launch costs the host (4 us) as much as the work takes.  Measured with events (some 5 us of them the
-// events'), words of falling frequency, against the three launches: 1280 words, 5000 x 512 fp32, 16.8 and 20.7 us; 2049 words, 432 x
-// 301 fp16, 16.6 and 26.0; 4096 words, 5000 x 512 fp32, 31.5 and 28.6, and 8 us less of the host.  Above SMALL_TABLE the
-// workgroups no longer run side by side, and the looking at all tokens shows: 256 words, 50000 x 1024 bf16, 48.3 and 27.4 us.
+// n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists
+// the positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than SMALL_ALONE positions
+// are left for all sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of
+// a sort, groups and rows: at these sizes a launch costs the host (4 us) as much as the work takes.  Measured with events (some
+// 5 us of them the events'), words of falling frequency, against the three launches: 1280 words, 5000 x 512 fp32, 16.8 and 20.7
+// us; 2049 words, 432 x 301 fp16, 16.6 and 26.0; 4096 words, 5000 x 512 fp32, 31.5 and 28.6, and 8 us less of the host.  Above
+// SMALL_TABLE the workgroups no longer run side by side, and the looking at all tokens shows: 256 words, 50000 x 1024 bf16,
+// 48.3 and 27.4 us.
 constexpr int SMALL_MAX = 4096;
 constexpr int SMALL_ROWS = 64;
 constexpr int64_t SMALL_TABLE = 1 << 23;   // elements: two workgroups of SMALL_ROWS rows and 256 columns for every CU
@@ -349,7 +351,8 @@ __device__ __forceinline__ void put_row(const SumArgs& a, int64_t v, int col, co
 }
 
 template <typename T, int N>
-__global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const SumArgs a, const void* tok, int tok64, int64_t pad, int rows) {
+__global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const SumArgs a, const void* tok, int tok64, int64_t pad,
+                                                                       int rows) {
   __shared__ unsigned s_list[SMALL_MAX];                     // row of the workgroup << 16 | position
   __shared__ unsigned s_pos[SMALL_WAVES][128];
   __shared__ float s_sum[SMALL_WAVES][64 * N];
@@ -360,7 +363,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const Sum
   const int col = lane_column<N>(blockIdx.x - unit * a.slices, a.width);
   const unsigned v0 = unit * (unsigned)rows, mine = a.vocab - v0 < (unsigned)rows ? a.vocab - v0 : (unsigned)rows;
   const T* dy = reinterpret_cast<const T*>(a.dy);
-  const int n = (int)a.n, each = (n + 64 * SMALL_WAVES - 1) / (64 * SMALL_WAVES) * 64;      // a wave looks at `each` tokens, 64 at a time
+  const int n = (int)a.n;
+  const int each = (n + 64 * SMALL_WAVES - 1) / (64 * SMALL_WAVES) * 64;      // a wave looks at `each` tokens, 64 at a time
   if (threadIdx.x < SMALL_ROWS) s_count[threadIdx.x] = 0;
   unsigned row[SMALL_MAX / (64 * SMALL_WAVES)];
 #pragma unroll
@@ -436,8 +440,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void token_small_kernel(const Sum
   }
 }
 
-// first sorted position i in [lo, n) with skey[i] >= v (RISE = 0), or skey[i] + i >= v (RISE = 1): 64 lanes look at 64 places at
-// a time
+// first sorted position i in [lo, n) with skey[i] >= v (RISE = 0), or skey[i] + i >= v (RISE = 1): 64 lanes look at 64 places
+// at a time
 template <int RISE>
 __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_t lo, int64_t n, unsigned v, int lane) {
   int64_t len = n - lo;                          // the answer is in [lo, lo + len]
@@ -455,13 +459,13 @@ __device__ __forceinline__ int64_t wave_lower_bound(const unsigned* skey, int64_
   return lo;
 }
 
-// The rows of the table, each followed by its sorted positions, are one sequence of vocab + n entries: row v is entry
-// v + (positions of smaller keys).  It is cut into stretches of STRETCH entries, and a wave owns the rows that lie in its
-// stretch (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows
-// without a position as zeros.  So no wave has much more to do than another, whatever the tokens are (equal numbers of rows a wave
-// took 394 us instead of 33 for 32768 words of falling frequency: the frequent ones lie side by side).  It walks 64 sorted
-// positions at a time; the dy rows of several tokens are on their way together.  Bound by dy and dw: 131072 x 2048 bf16 of
-// each, 176 us, 4.6 TB/s of what is left of dy and dw.
+// The rows of the table, each followed by its sorted positions, are one sequence of vocab + n entries: row v is entry v +
+// (positions of smaller keys).  It is cut into stretches of STRETCH entries, and a wave owns the rows that lie in its stretch
+// (and 64 * N columns): it adds up their positions - fewer than 64 behind the stretch's end - and writes them, rows without a
+// position as zeros.  So no wave has much more to do than another, whatever the tokens are (equal numbers of rows a wave took
+// 394 us instead of 33 for 32768 words of falling frequency: the frequent ones lie side by side).  It walks 64 sorted positions
+// at a time; the dy rows of several tokens are on their way together.  Bound by dy and dw: 131072 x 2048 bf16 of each, 176 us,
+// 4.6 TB/s of what is left of dy and dw.
 template <typename T, int N, bool PAST>
 __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
   const unsigned id = wave_id(), unit = id / a.slices;
@@ -525,7 +529,8 @@ __global__ __launch_bounds__(256) void token_rows_kernel(const SumArgs a) {
       const int64_t h1 = (g1 + GROUP - 1) / GROUP, h2 = g2 / GROUP;               // whole groups of groups
       const bool two = h1 < h2;
       for (int k = 0; k < 3; ++k) {              // groups before, groups of groups, groups behind them
-        const int64_t from = k == 0 ? g1 : k == 1 ? h1 : two ? h2 * GROUP : g2, to = k == 0 ? (two ? h1 * GROUP : g2) : k == 1 ? (two ? h2 : h1) : g2;
+        const int64_t from = k == 0 ? g1 : k == 1 ? h1 : two ? h2 * GROUP : g2;
+        const int64_t to = k == 0 ? (two ? h1 * GROUP : g2) : k == 1 ? (two ? h2 : h1) : g2;
         add_partials<N>(k == 1 ? a.part2 : a.part1, a.width, from, to, col, s);
       }
       finish(first, true);
@@ -617,9 +622,10 @@ int launch_fwd(const void* tok, int tok64, int64_t n, const void* table, int64_t
   const int64_t waves = (many ? (n + 3) / 4 : n) * slices;
   if (waves > MAX_WAVES) return GVD_EINVAL;
   const bool past = n * width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
-  hipLaunchKernelGGL((!many ? embedding_fwd_kernel<T, N, 1, false> : past ? embedding_fwd_kernel<T, N, 4, true> : embedding_fwd_kernel<T, N, 4, false>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
-                     st, tok, tok64, n, reinterpret_cast<const T*>(table), ld, (unsigned)vocab, width, scale, act,
-                     reinterpret_cast<T*>(out), ldo, slices);
+  const auto kernel = !many ? embedding_fwd_kernel<T, N, 1, false>
+                      : past ? embedding_fwd_kernel<T, N, 4, true> : embedding_fwd_kernel<T, N, 4, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, tok, tok64, n, reinterpret_cast<const T*>(table),
+                     ld, (unsigned)vocab, width, scale, act, reinterpret_cast<T*>(out), ldo, slices);
   GVD_CHECK_LAUNCH();
   return 0;
 }
@@ -652,7 +658,8 @@ template <typename T, int N> int launch_sums(SumArgs a, hipStream_t st) {
     GVD_CHECK_LAUNCH();
   }
   const bool past = (int64_t)a.vocab * a.width * (int64_t)sizeof(T) > GVD_CACHE_BYTES;
-  hipLaunchKernelGGL((past ? token_rows_kernel<T, N, true> : token_rows_kernel<T, N, false>), dim3((unsigned)((owners + 3) / 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((past ? token_rows_kernel<T, N, true> : token_rows_kernel<T, N, false>), dim3((unsigned)((owners + 3) / 4)),
+                     dim3(256), 0, st, a);
   GVD_CHECK_LAUNCH();
   return 0;
 }
@@ -691,8 +698,8 @@ extern "C" size_t gvd_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, in
   return (size_t)bwd_space(n, vocab, width).bytes;
 }
 
-extern "C" int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const void* dy, int64_t ld_dy, const void* table, int64_t ld,
-                                 int64_t vocab, int width, int dtype, float scale, int act, int64_t padding_idx, void* dw,
+extern "C" int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const void* dy, int64_t ld_dy, const void* table,
+                                 int64_t ld, int64_t vocab, int width, int dtype, float scale, int act, int64_t padding_idx, void* dw,
                                  void* workspace, size_t workspace_bytes, gvd_stream_t stream) {
   if (!tokens || !dy || !dw || bad_shape(n, vocab, width, dtype) || ld_dy < 0 || (act && (!table || ld < width)))
     return GVD_EINVAL;

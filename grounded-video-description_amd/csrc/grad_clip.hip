@@ -8,10 +8,10 @@
 // fixed order (no atomics).  Two kinds of launch: gvd_grad_sumsq leaves one partial sum per workgroup; in gvd_grad_scale every
 // workgroup adds up all the partials by itself, in the same order, so no launch is spent on joining them.
 //
-// Measured, 100 tensors of 2.5 M elements bf16 -> fp32: norm 84 us (6.0 TB/s), both 312 us; 10 tensors of 4 M fp32: 30 and 82 us.
-// What got it there from 128 + 294 us: a whole chunk in flight before its first use, stores and second reads past the cache
-// (394 -> 330 us), eight workgroups of the second pass for each resident one (330 -> 312), destinations taken from their 128-byte
-// lines on (views of a flat buffer at odd offsets: 368 -> 332).
+// Measured, 100 tensors of 2.5 M elements bf16 -> fp32: norm 84 us (6.0 TB/s), both 312 us; 10 tensors of 4 M fp32: 30 and 82
+// us. What got it there from 128 + 294 us: a whole chunk in flight before its first use, stores and second reads past the cache
+// (394 -> 330 us), eight workgroups of the second pass for each resident one (330 -> 312), destinations taken from their
+// 128-byte lines on (views of a flat buffer at odd offsets: 368 -> 332).
 //
 // Up to GVD_GRAD_MAX_TENSORS tensors go into a launch by value (addresses and sizes in the kernel's arguments); a workgroup
 // finds the tensor of its chunk by bisection in the chunk counts.
@@ -120,8 +120,8 @@ __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, F
   for (int64_t i = nv + threadIdx.x; i < n; i += 256) dst[i] = (TO)((float)src[i] * f.f * f.p);
 }
 
-// Chunk k of a tensor.  Its chunks begin where the destination begins a 128-byte line (the first one holds what lies before, too):
-// results that are views of a flat buffer begin anywhere, and stores of parts of lines cost more than such loads.
+// Chunk k of a tensor.  Its chunks begin where the destination begins a 128-byte line (the first one holds what lies before,
+// too): results that are views of a flat buffer begin anywhere, and stores of parts of lines cost more than such loads.
 template <bool PAST, typename TI, typename TO>
 __device__ __forceinline__ void scale_chunk(const TI* src, TO* dst, int64_t k, int64_t n, Factor f) {
   const int64_t before = (int64_t)((128u - (unsigned)(reinterpret_cast<uintptr_t>(dst) & 127u)) % 128u / sizeof(TO));

@@ -1957,7 +1957,7 @@ def beam_select(logits, scores, width=None, finished=None, eos=None):
 
     logits [B*K, V] or [B, K, V], fp32 / bf16 / fp16, contiguous rows (any row stride); scores f32 [B, K] (the beams' summed
     log-probabilities; -inf: not in use yet); width: K unless given.  finished (u8 / bool [B, K]): an ended beam goes on with
-    the word `eos` at its score and nothing else; its logits are not read.  A beam whose score or log-sum-exp is not finite
+    the word `eos` at its score and nothing else; its logits do not matter.  A beam whose score or log-sum-exp is not finite
     (NaN or +inf logits, all words banned) has -inf for every word.  Candidates are scored and compared in fp64.
 
     Returns (scores f32 [B, W], parent i64 [B, W], word i64 [B, W], finished [B, W]): parent = the row b*K + q the candidate

@@ -757,8 +757,8 @@ int gvd_grad_scale(const gvd_grad_group* g, const gvd_grad_clip* c, const void* 
 /* Beam search's selection of one step: for each of B samples the W best of the K * V candidates
  *   cand[q,v] = scores[b,q] + (logits[b*K+q, v] - log sum_v exp(logits[b*K+q, v]))
  * in descending order, equal ones by q * V + v ascending, computed and compared in fp64 (words of one beam: by their logits).
- * finished (nullable, u8 [B,K]): an ended beam has scores[b,q] for the word eos and -inf for the others; its logits are not
- * read.  A beam whose score or log-sum-exp is not finite has -inf for every word.  logits [B*K, V] of type dtype, row stride ld.
+ * finished (nullable, u8 [B,K]): an ended beam has scores[b,q] for the word eos and -inf for the others; its logits do
+ * not matter.  A beam whose score or log-sum-exp is not finite has -inf for every word.  logits [B*K, V] of type dtype, row stride ld.
  * Out, [B,W] each: out_scores f32, parent = b*K + q, word, out_finished = finished[b,q] or word == eos (nullable; eos = -1: none).
  * Limits: K, W <= GVD_BEAM_SELECT_MAX, W <= K * V, B * K <= 65535, V <= 2^28.
  * workspace: gvd_beam_select_workspace_bytes(B, K, V, W) bytes, 16-byte aligned, contents free. */
