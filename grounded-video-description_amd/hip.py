@@ -354,6 +354,14 @@ def run_on(device, fn, what, *args):
         check(rc, what)
 
 
+def written(tensors):
+    """Tell autograd's version counters that kernels wrote these tensors through raw pointers."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                                 # (inference tensors have no version)
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def ptr(t):
     """Device pointer of a tensor (None -> NULL)."""
     if t is None:

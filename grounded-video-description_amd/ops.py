@@ -9,6 +9,7 @@ import torch
 
 from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs, DxGroup, GemmArgs, GemmSeg, GreedyArgs,
                   GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr, require_cuda_f32, run_on, stream_ptr)
+from .hip import written as mark_written
 
 # ---------------------------------------------------------------------------------------------------------------------
 # "No library GEMM on the hot path" as an invariant.  Every place where a product or softmax of the path would leave
@@ -1962,7 +1963,7 @@ def beam_select(logits, scores, width=None, finished=None, eos=None):
 
     Returns (scores f32 [B, W], parent i64 [B, W], word i64 [B, W], finished [B, W]): parent = the row b*K + q the candidate
     extends, as reorder_rows takes it; finished = of the type given (u8 if none was), None without eos.
-    K, W <= 32; B * K <= 65535."""
+    K, W <= 32; B * K <= 65535.  Not differentiable."""
     if logits.dtype not in DTYPES or scores.dtype != torch.float32 or scores.dim() != 2:
         raise GvdHipError('beam_select: logits must be float32 / bfloat16 / float16 and scores float32 [B, K], got %s and %s %s'
                           % (logits.dtype, scores.dtype, tuple(scores.shape)))
@@ -2053,7 +2054,8 @@ def reorder_rows(states, parent, dim=0, out=None):
     states: tensors of any type whose dimension `dim` holds the same number of rows; parent int64, any shape (its entries in
     order are the new rows: beam_select's parent goes in as it is).  out: tensors of the result's shape and type, which must not
     overlap the states (two sets of buffers, swapped from step to step); otherwise new ones.  Returns the list of results.
-    A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1)."""
+    A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1).  Not
+    differentiable: the results carry no gradient."""
     states = list(states)
     dev = parent.device
     if parent.dtype != torch.int64:
@@ -2124,4 +2126,6 @@ def reorder_rows(states, parent, dim=0, out=None):
             t.src, t.dst, t.outer = x.data_ptr(), y.data_ptr(), outer
             t.src_outer, t.dst_outer, t.src_row, t.dst_row, t.row_bytes = so, do, sr, dr, row
         run_on(dev, lib().gvd_reorder_rows, 'gvd_reorder_rows', C.byref(g), parent.data_ptr(), rows, n)
+    if out is not None:
+        mark_written(results)
     return results

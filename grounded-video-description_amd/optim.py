@@ -14,6 +14,7 @@ import operator
 import numpy as np
 import torch
 
+from . import hip
 from .hip import (DTYPES, GRAD_CHUNK, GRAD_MAX_TENSORS, OPT_CHUNK, OPT_MAX_TENSORS, GradClip, GradGroup, GvdHipError, OptGroup, check,
                   lib, ptr, run_on, stream_ptr)
 
@@ -373,10 +374,7 @@ def clip_grads(grads, max_norm, out=None, inv_scale=1.0, error_if_nonfinite=Fals
     norm = _norm_and_scale(device, s, d, max_norm, inv_scale, error_if_nonfinite, what)
     for o, x in back:
         o.copy_(x)
-    try:
-        torch.autograd.graph.increment_version(written)
-    except RuntimeError:                                 # (inference tensors have no version)
-        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    hip.written(written)
     return norm
 
 

@@ -154,6 +154,15 @@ def test_embedding_strides(dtype):
     check_embedding(tok, one.expand(V, E), 1.0, 0, what='broadcast table')
 
 
+def test_embedding_of_one_token():
+    w = torch.randn(9, 6, device='cuda', requires_grad=True)
+    for t in (torch.tensor(3, device='cuda'), torch.tensor([3], device='cuda', dtype=torch.int32)):
+        out = ops.embedding(t, w, scale=2.0)
+        assert out.shape == t.shape + (6,) and torch.equal(out.detach().view(-1), w.detach()[3] * 2)
+        g, = torch.autograd.grad(out.sum(), w)
+        assert float(g.sum()) == 12.0 and float(g[3].sum()) == 12.0
+
+
 def test_embedding_of_nothing():
     w = torch.randn(9, 6, device='cuda', requires_grad=True)
     out = ops.embedding(torch.zeros(0, 4, dtype=torch.int64, device='cuda'), w)
@@ -580,6 +589,15 @@ def test_reorder_refuses_shared_memory():
         with pytest.raises(hip.GvdHipError):
             ops.reorder_rows(states, p, out=out)
     ops.reorder_rows([x, x], p, out=[o, torch.empty_like(o)])
+
+
+def test_reorder_into_a_saved_tensor_is_seen_by_autograd():
+    w = torch.ones(4, 3, device='cuda', requires_grad=True)
+    buf = torch.ones(4, 3, device='cuda')
+    y = (w * buf).sum()                           # saves buf
+    ops.reorder_rows([torch.zeros(4, 3, device='cuda')], torch.arange(4, device='cuda'), out=[buf])
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
 
 
 def test_reorder_rows_outside_and_nothing():
