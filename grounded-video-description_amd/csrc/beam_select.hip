@@ -79,6 +79,11 @@ __device__ __forceinline__ unsigned wave_bound(unsigned x, int W) {
   return t;
 }
 
+__device__ __forceinline__ float least_of(u64 floor) {
+  const unsigned bits = (unsigned)(floor >> 32);
+  return bits > 0x007fffffu ? from_order_bits(bits) : -INFINITY;
+}
+
 __device__ __forceinline__ int lanes_below(u64 mask, int lane) { return __popcll(mask & ((1ull << lane) - 1ull)); }
 
 // the best W of the n words on a wave's list, in order, to its front: every word counts those before it
@@ -165,11 +170,16 @@ void beam_part_kernel(const SelectArgs a) {
 #pragma unroll
     for (int i = 0; i < IPT; ++i) s[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * 1.44269504088896341f);
     sum = sum * (double)__builtin_amdgcn_exp2f((was - ref) * 1.44269504088896341f) + (double)((s[0] + s[1]) + (s[2] + s[3]));
-    if (v0 == first) floor = (u64)wave_bound(order_bits(mx), W) << 32;
-    // no word under `least` is among the best (bits under those of -inf are no number)
-    const unsigned bits = (unsigned)(floor >> 32);
-    const float least = bits > 0x007fffffu ? from_order_bits(bits) : -INFINITY;
-    if (!__ballot(mx >= least)) continue;
+    // no word under `least` is among the best (bits under those of -inf are no number).  Where W lanes or more have one over it -
+    // the first tile, rising logits - what W lanes reach in this tile raises it
+    float least = least_of(floor);
+    const u64 lanes = __ballot(mx >= least);
+    if (!lanes) continue;
+    if (__popcll(lanes) >= W) {
+      const u64 reached = (u64)wave_bound(order_bits(mx), W) << 32;
+      floor = reached > floor ? reached : floor;
+      least = least_of(floor);
+    }
     unsigned todo = 0;                     // the lane's words at or over it
 #pragma unroll
     for (int i = 0; i < IPT; ++i) todo |= v[i] >= least ? 1u << i : 0u;

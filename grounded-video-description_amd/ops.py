@@ -7,8 +7,9 @@ import os
 
 import torch
 
-from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs, DxGroup, GemmArgs, GemmSeg, GreedyArgs,
-                  GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr, require_cuda_f32, run_on, stream_ptr)
+from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs,
+                  DxGroup, GemmArgs, GemmSeg, GreedyArgs, GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr,
+                  require_cuda_f32, run_on, stream_ptr)
 from .hip import written as mark_written
 
 # ---------------------------------------------------------------------------------------------------------------------
