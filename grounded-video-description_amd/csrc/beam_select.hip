@@ -328,15 +328,21 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(const SelectArgs a) {
 struct SelectShape { int ipt, parts, tiles_per_part; };
 
 SelectShape select_shape(int64_t rows, int V, int W, int dtype) {
-  SelectShape s;
+  // parts that fill the device (16 waves a CU), and the tile that a wave gets through its part with soonest: a tile of i logits a
+  // lane costs some 24 + i (its bound and its ranking as much as 24 logits).  15 x 12 beams, 32003 words fp16: one tile of 32 a wave,
+  // two of 16 10.5 us, three of 8 12.5; 64 x 5 beams, 5000 words fp32: one of 8 5.9 us, two of 4 6.9.
   const int least = dtype == GVD_F32 ? 4 : 8;
   int64_t most = MAX_PARTS < JOIN_LIST / W ? MAX_PARTS : JOIN_LIST / W;
   if (most > 4096 / rows) most = 4096 / rows > 1 ? 4096 / rows : 1;
-  s.ipt = 32;
-  while (s.ipt > least && ((V + 64 * s.ipt - 1) / (64 * s.ipt) < most || 32 * s.ipt >= V)) s.ipt /= 2;
-  const int tiles = (V + 64 * s.ipt - 1) / (64 * s.ipt);
-  s.tiles_per_part = (int)((tiles + most - 1) / most);
-  s.parts = (tiles + s.tiles_per_part - 1) / s.tiles_per_part;
+  SelectShape s = {0, 0, 0};
+  int64_t cost = 0;
+  for (int ipt = 32; ipt >= least; ipt /= 2) {
+    if (ipt > least && 32 * ipt >= V) continue;              // (half of the tile would do)
+    const int tiles = (V + 64 * ipt - 1) / (64 * ipt), per_part = (int)((tiles + most - 1) / most);
+    if (s.ipt && (int64_t)per_part * (24 + ipt) >= cost) continue;
+    cost = (int64_t)per_part * (24 + ipt);
+    s = {ipt, (tiles + per_part - 1) / per_part, per_part};
+  }
   return s;
 }
 
