@@ -6,10 +6,11 @@
 //                                      a beam that is not in use yet): -inf for all words
 //   the `width` largest of the K * V candidates of a sample, descending, equal ones by q * V + v ascending
 //
-// Bound by the logits, which are read once: one launch walks them with the running maximum and sum of the softmax and keeps the
-// `width` best of each part of a row, a second one joins the parts and the beams of a sample.  The best words of a row are its
-// largest logits, so the walk compares logits; only the join, a few candidates per beam, needs scores, and computes them in
-// fp64: two beams' candidates may lie closer together than fp32 tells apart.
+// One launch walks the logits, once, with the running maximum and sum of the softmax and keeps the `width` best of each part of a
+// row, a second one joins the parts and the beams of a sample.  The best words of a row are its largest logits, so the walk
+// compares logits.  Two beams' candidates may lie closer together than fp32 tells apart, and their order hangs on the beams'
+// log-sum-exps: exponentials, sums, logarithm and candidates are fp64 throughout (good to some 1e-14; with fp32 exponentials, 1e-7,
+// beams closer than that came out in either order).
 #include "dtypes.h"
 #include <math.h>
 
@@ -115,11 +116,12 @@ __device__ __forceinline__ void rank_list(u64* list, int n, int W, int lane) {
 // One wave per part of a row: 64 * IPT logits at a time, the next ones on their way meanwhile.  Every lane has a running
 // maximum and sum of its own.  A word goes on the list if it beats the W-th best so far (key `floor`); at the start that is a
 // value that the maxima of W lanes reach.  The list is ranked, and the floor raised, behind a tile and when it is full; logits
-// of any order and equality only make that more frequent.  A wave works by itself, without a barrier: 256 rows of 131072 bf16
-// logits take 29 us (the hits of the list are 6 of them, the exponentials none: loads and latency bound it), 256 rows fp32 30
-// us (4.0 TB/s), 5 rows of 5000 fp32 4.3 us.  The same with a workgroup per part, barriers and a list of its own: 66 us.  Code
-// is kept small (a lane finds its next word by selecting, not by 32 copies of the append): at one tile a wave, fetching 50 KB
-// of instructions was most of the time.
+// of any order and equality only make that more frequent.  A wave works by itself, without a barrier.  Bound by the fp64
+// exponentials, some 25 full-rate instructions each: 256 rows of 131072 bf16 logits take 52 us (2^x in fp32: 29 us, and the order
+// of close beams wrong), 320 rows of 5000 fp32 8.2 us (5.9), 5 rows 4.7 us (4.4).  A series written out here instead of exp()
+// is 3 % faster.  A workgroup per part, with barriers and a list of its own, took twice the time of the waves.  Code is kept small
+// (a lane finds its next word by selecting, not by 32 copies of the append): at one tile a wave, fetching 50 KB of instructions
+// was most of the time.
 template <typename T, int IPT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(IPT == 32 && sizeof(T) == 2 ? 4 : 3)))
 void beam_part_kernel(const SelectArgs a) {
@@ -162,14 +164,14 @@ void beam_part_kernel(const SelectArgs a) {
 #pragma unroll
     for (int i = 0; i < IPT; ++i) { v[i] = (float)next[i / N][i % N]; mx = fmaxf(mx, v[i]); }
     if (v0 + TILE < end) fetch(v0 + TILE);
-    // softmax: terms 2^((x - top) log2 e) on v_exp_f32; nothing but -inf so far: every term is 0
+    // softmax in fp64, as the candidates are compared; nothing but -inf so far: every term is 0
     const float was = top;
     top = fmaxf(top, mx);
-    const float ref = top > -INFINITY ? top : 0.f;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const double ref = top > -INFINITY ? (double)top : 0.0;
+    double s[2] = {0.0, 0.0};
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) s[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * 1.44269504088896341f);
-    sum = sum * (double)__builtin_amdgcn_exp2f((was - ref) * 1.44269504088896341f) + (double)((s[0] + s[1]) + (s[2] + s[3]));
+    for (int i = 0; i < IPT; ++i) s[i & 1] += exp((double)v[i] - ref);
+    sum = sum * exp((double)was - ref) + (s[0] + s[1]);
     // no word under `least` is among the best (bits under those of -inf are no number).  Where W lanes or more have one over it -
     // the first tile, rising logits - what W lanes reach in this tile raises it
     float least = least_of(floor);
@@ -207,7 +209,7 @@ void beam_part_kernel(const SelectArgs a) {
   }
   // the lanes' sums, each to its own maximum, into one (NaN and +inf go through to the join, which drops the beam)
   const float all = wave_max_f32(top);
-  sum = gvd_wave_sum_f64(sum != 0.0 ? sum * (double)__builtin_amdgcn_exp2f((top - all) * 1.44269504088896341f) : 0.0);
+  sum = gvd_wave_sum_f64(sum != 0.0 ? sum * exp((double)top - (double)all) : 0.0);
   const int64_t rec = (int64_t)row * a.parts + part;
   if (lane == 0) a.stat[rec] = make_double2((double)all, sum);
   if (lane < W) a.best[rec * W + lane] = list[lane];
@@ -329,8 +331,9 @@ struct SelectShape { int ipt, parts, tiles_per_part; };
 
 SelectShape select_shape(int64_t rows, int V, int W, int dtype) {
   // parts that fill the device (16 waves a CU), and the tile that a wave gets through its part with soonest: a tile of i logits a
-  // lane costs some 24 + i (its bound and its ranking as much as 24 logits).  15 x 12 beams, 32003 words fp16: one tile of 32 a wave,
-  // two of 16 10.5 us, three of 8 12.5; 64 x 5 beams, 5000 words fp32: one of 8 5.9 us, two of 4 6.9.
+  // lane costs some 24 + i (its bound and its ranking as much as 24 logits).  Both launches, with events: 15 x 12 beams, 32003 words
+  // fp16: one tile of 32 a wave 30 us, two of 16 31.5, three of 8 35; 64 x 5 beams, 5000 words fp32: one of 8 19.2 us, of 16 20, two
+  // of 4 20.4.
   const int least = dtype == GVD_F32 ? 4 : 8;
   int64_t most = MAX_PARTS < JOIN_LIST / W ? MAX_PARTS : JOIN_LIST / W;
   if (most > 4096 / rows) most = 4096 / rows > 1 ? 4096 / rows : 1;

@@ -1,0 +1,51 @@
+"""-m gpu: edges of the token-side operators - beams that lie closer together than fp32 tells apart."""
+import pytest
+import torch
+
+from gvd_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ids = lambda t: str(t).replace('torch.', '')      # noqa: E731
+
+
+def gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------------------------------------ beam_select
+def select_want(logits, scores, W):
+    """The definition in 64 bits: beams and words of the best W, and the least distance between neighbours of different beams among
+    the best W + 1."""
+    B, K = scores.shape
+    x = logits.double().view(B, K, -1)
+    V = x.shape[2]
+    m = x.max(dim=2, keepdim=True)[0]
+    cand = scores.double().unsqueeze(2) + (x - (m + (x - m).exp().sum(2, keepdim=True).log()))
+    best, at = cand.view(B, K * V).sort(dim=1, descending=True, stable=True)
+    best, at = best[:, :W + 1], at[:, :W + 1]
+    gap = torch.where(at[:, :W] // V != at[:, 1:] // V, best[:, :W] - best[:, 1:], torch.ones((), device='cuda', dtype=torch.float64))
+    return at[:, :W] // V, at[:, :W] % V, gap.min(dim=1)[0]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+@pytest.mark.parametrize('V', [3, 50, 700, 5000, 70001])
+def test_beam_select_orders_beams_that_are_close(V, dtype):
+    """Every beam's score is set so that its best word comes out where the first beam's does, but for the score's rounding to fp32 (up
+    to some 1e-7 between beams): the order is the definition's.  Both sides hold the log-sum-exp in fp64, to some 1e-14 (a relative
+    error of a few 2^-53 in every term, all of one sign, and in the logarithm); pairs of beams closer than 1e-12 are left out, and
+    there are hardly any."""
+    B, K = 64, 4
+    x = (torch.randn(B * K, V, generator=gen(V), device='cuda') * 3).to(dtype)
+    lp = x.double().log_softmax(dim=1).max(dim=1)[0].view(B, K)
+    scores = (lp[:, :1] - lp).float()
+    for W in (K, 1):
+        beam, word, gap = select_want(x, scores, W)
+        _, parent, got, _ = ops.beam_select(x, scores, width=W)
+        apart = gap > 1e-12
+        assert int(apart.sum()) > 0.9 * B
+        first = torch.arange(B, device='cuda').unsqueeze(1) * K
+        assert torch.equal((parent - first)[apart], beam[apart]) and torch.equal(got[apart], word[apart])
+        places = (parent * V + got).sort(dim=1)[0]
+        assert bool((places[:, 1:] > places[:, :-1]).all())                       # no candidate twice
