@@ -2054,7 +2054,7 @@ def reorder_rows(states, parent, dim=0, out=None):
 
     states: tensors of any type whose dimension `dim` holds the same number of rows; parent int64, any shape (its entries in
     order are the new rows: beam_select's parent goes in as it is).  out: tensors of the result's shape and type, which must not
-    overlap the states (two sets of buffers, swapped from step to step); otherwise new ones.  Returns the list of results.
+    overlap the states or parent (two sets of buffers, swapped from step to step); otherwise new ones.  Returns the list of results.
     A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1).  Not
     differentiable: the results carry no gradient."""
     states = list(states)
@@ -2109,16 +2109,17 @@ def reorder_rows(states, parent, dim=0, out=None):
             if not ok:
                 raise GvdHipError('reorder_rows: result %d is not made of whole rows of their own (strides %s)' % (i, y.stride()))
         items.append((x, y, src, dst))
-    if not parent.is_cuda:
-        raise GvdHipError('reorder_rows: non-GPU tensor; there is no CPU fallback')
-    if out is not None:
-        spans = sorted([_extent(y) + (1,) for _, y, _, _ in items] + [_extent(x) + (0,) for x, _, _, _ in items])
+    if out is not None and items:
+        spans = sorted([_extent(y) + (1,) for _, y, _, _ in items] + [_extent(x) + (0,) for x, _, _, _ in items]
+                       + [_extent(parent) + (0,)])
         end, wend = 0, 0
         for a, b, written in spans:                  # (states may overlap each other; a result may overlap nothing)
             if a < wend or written and a < end:
-                raise GvdHipError('reorder_rows: a result overlaps a state or another result')
+                raise GvdHipError('reorder_rows: a result overlaps a state, the parents or another result')
             end = max(end, b)
             wend = max(wend, b) if written else wend
+    if not parent.is_cuda:
+        raise GvdHipError('reorder_rows: non-GPU tensor; there is no CPU fallback')
     for k in range(0, len(items), REORDER_MAX_TENSORS):
         part = items[k:k + REORDER_MAX_TENSORS]
         g = ReorderGroup()

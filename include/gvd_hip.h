@@ -776,8 +776,8 @@ int gvd_beam_select(const gvd_beam_select_args* args, gvd_stream_t stream);
 
 /* Reordering of the beams' states: dst[o, r, :] = src[o, index[r], :] for up to GVD_REORDER_MAX_TENSORS tensors in one launch.
  * A tensor is [outer, rows, row_bytes] with the byte strides src_outer / src_row and dst_outer / dst_row; index int64
- * [rows_out], shared by the tensors.  src and dst must not overlap.  An index outside [0, rows_in) reads nothing: its
- * rows get all bits set (NaN, -1).  `unit` and `tile0` are filled in by the call. */
+ * [rows_out], shared by the tensors.  A dst must not overlap a src, the index or another dst.  An index outside [0, rows_in) reads
+ * nothing: its rows get all bits set (NaN, -1).  `unit` and `tile0` are filled in by the call. */
 #define GVD_REORDER_MAX_TENSORS 16
 typedef struct {
   const void* src; void* dst;

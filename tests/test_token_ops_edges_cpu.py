@@ -1,0 +1,18 @@
+"""CPU: calls of the token-side operators that are refused before a GPU is touched, and the rules of their C entries' workspaces."""
+import pytest
+import torch
+
+from gvd_amd import hip, ops
+
+
+def test_reorder_refuses_a_result_over_its_index():
+    """One workgroup would write the index while another still reads it."""
+    words = torch.zeros(6, dtype=torch.int64)
+    buf = torch.zeros(3, 6, dtype=torch.int64)
+    for parent, out in ((words, words), (words.view(2, 3), words.view(-1)), (buf[1], buf[1]), (buf.view(-1)[4:10], buf[1])):
+        with pytest.raises(hip.GvdHipError, match='overlaps'):
+            ops.reorder_rows([torch.ones(6, dtype=torch.int64)], parent, out=[out])
+    # apart from the result, or copied before the launch (its entries do not lie side by side): as far as the check of the device
+    for parent in (buf[0], buf[2], buf.t()[0].repeat(2), buf.t()[:2].reshape(-1)):
+        with pytest.raises(hip.GvdHipError, match='no CPU fallback'):
+            ops.reorder_rows([torch.ones(6, dtype=torch.int64)], parent, out=[buf[1]])
