@@ -6,6 +6,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from .hip import (BEAM_SELECT_MAX, DTYPES, EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, REORDER_MAX_TENSORS, AttnSide, BeamSelectArgs,
                   DxGroup, GemmArgs, GemmSeg, GreedyArgs, GvdHipError, LstmArgs, ReorderGroup, check, lib, ptr,
@@ -1876,6 +1877,8 @@ def _check_embedding(tokens, weight, act, padding_idx):
                           % (EMBEDDING_MAX, EMBEDDING_MAX_WIDTH, tokens.numel(), tuple(weight.shape)))
     if not V and tokens.numel():
         raise GvdHipError('embedding: the table has no rows')
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(weight).tangent is not None:
+        raise GvdHipError('embedding: the table carries a forward-mode tangent; there is a reverse-mode gradient only')
     if not (tokens.is_cuda and weight.is_cuda):
         raise GvdHipError('embedding: non-GPU tensor; there is no CPU fallback')
     if tokens.device != weight.device:
@@ -1935,7 +1938,7 @@ _embedding_bwd_once = torch.autograd.function.once_differentiable(_embedding_bwd
 
 def embedding(tokens, weight, scale=1.0, act=0, padding_idx=None):
     """act(scale * weight[tokens]) - the word embedding with its scaling and ReLU (model.py:79-82: Embedding + ReLU) in one
-    launch, differentiable with respect to `weight`.
+    launch, differentiable with respect to `weight` once, in reverse mode.
 
     tokens int64 / int32 of any shape, weight [V, E] fp32 / bf16 / fp16 (a column block of a wider table is read in place);
     act 1 = ReLU; padding_idx: a row that gets no gradient.  The result has weight's type, [..., E], rounded once.

@@ -16,3 +16,19 @@ def test_reorder_refuses_a_result_over_its_index():
     for parent in (buf[0], buf[2], buf.t()[0].repeat(2), buf.t()[:2].reshape(-1)):
         with pytest.raises(hip.GvdHipError, match='no CPU fallback'):
             ops.reorder_rows([torch.ones(6, dtype=torch.int64)], parent, out=[buf[1]])
+
+
+def test_embedding_refuses_a_table_with_a_tangent():
+    """There is no forward-mode rule: a tangent is refused, not lost, whether or not the table requires a gradient too."""
+    import torch.autograd.forward_ad as fw
+    tok, w = torch.zeros(3, dtype=torch.int64), torch.randn(7, 4)
+    with fw.dual_level():
+        for grad in (False, True):
+            dual = fw.make_dual(w.clone().requires_grad_(grad), torch.ones(7, 4))
+            for table in (dual, dual[:, 1:3], dual.t().contiguous().t()):
+                with pytest.raises(hip.GvdHipError, match='forward-mode'):
+                    ops.embedding(tok, table)
+        with pytest.raises(hip.GvdHipError, match='no CPU fallback'):
+            ops.embedding(tok, w)                   # no tangent: as far as the check of the device
+    with pytest.raises(hip.GvdHipError, match='forward-mode'):
+        torch.func.jvp(lambda t: ops.embedding(tok, t), (w,), (w,))
