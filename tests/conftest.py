@@ -17,6 +17,13 @@ def pytest_configure(config):
     config.addinivalue_line('markers', 'gpu: needs a real MI355X (run with `-m gpu` on the GPU box)')
 
 
+def pytest_collection_modifyitems(items):
+    """The knob tests go first: their child processes launch cooperatively, and a process that has made such a launch keeps its
+    cooperative queue until it ends.  Where the machine grants one process at a time such a queue, the children of a process that
+    holds it (the bi-GRU tests with the library grid sync launch that way) get hipError 401.  Everything else keeps its order."""
+    items.sort(key=lambda item: os.path.basename(str(item.fspath)) != 'test_gpu_knobs.py')
+
+
 @pytest.fixture(scope='session')
 def golden_dir():
     return os.path.join(ROOT, 'tests', 'golden')
