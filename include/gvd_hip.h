@@ -722,7 +722,8 @@ int gvd_embedding_fwd(const void* tokens, int tok64, int64_t n, const void* tabl
  * contiguous dw [vocab, width] written once (tokens not met, and row padding_idx, as zeros; -1 = no padding row); tokens
  * outside [0, vocab) add nothing.  dy [n, width] with row stride ld_dy (0 = one row for all).  table is read for act = 1 only.
  * Positions are sorted by token and summed in fp32 in a fixed order: no atomics, the same bits at every run.
- * workspace: gvd_embedding_bwd_workspace_bytes(n, vocab, width) bytes (0 for n <= 4096), 16-byte aligned, contents free. */
+ * workspace: gvd_embedding_bwd_workspace_bytes(n, vocab, width) bytes, 16-byte aligned, contents free (0: none is needed; few
+ * tokens of a table that is not too large.  Ask the function: fewer bytes than it says, or NULL, are refused). */
 size_t gvd_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int width);
 int gvd_embedding_bwd(const void* tokens, int tok64, int64_t n, const void* dy, int64_t ld_dy, const void* table, int64_t ld,
                       int64_t vocab, int width, int dtype, float scale, int act, int64_t padding_idx, void* dw, void* workspace,

@@ -32,3 +32,15 @@ def test_embedding_refuses_a_table_with_a_tangent():
             ops.embedding(tok, w)                   # no tangent: as far as the check of the device
     with pytest.raises(hip.GvdHipError, match='forward-mode'):
         torch.func.jvp(lambda t: ops.embedding(tok, t), (w,), (w,))
+
+
+def test_embedding_workspace_is_what_the_function_says():
+    """Few tokens alone do not make it 0: with a large table the gradient is refused without it, before anything is launched."""
+    import ctypes as C
+    l, a = hip.lib(), C.c_void_p(4096)
+    for n, vocab, width in ((1, 70001, 129), (4096, 50000, 1024)):
+        need = l.gvd_embedding_bwd_workspace_bytes(n, vocab, width)
+        assert need > 0
+        for ws, size in ((None, need), (a, need - 1), (None, 0)):
+            assert l.gvd_embedding_bwd(a, 1, n, a, width, a, width, vocab, width, 0, 1.0, 0, -1, a, ws, size, None) == -1
+    assert l.gvd_embedding_bwd_workspace_bytes(4096, 5000, 512) == 0 == l.gvd_embedding_bwd_workspace_bytes(1, 1, 1)
