@@ -5,7 +5,7 @@
 //
 // (act' depends on the table row alone, so it multiplies the finished sum once.)  Both directions are bound by the rows they
 // move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable;
-// up to 4096 are listed by token instead), every row of dW is summed by one owner in a fixed order and written once, rows
+// few, of a small table, are listed by token instead), every row of dW is summed by one owner in a fixed order and written once, rows
 // without a token as zeros.  Sums are fp32.
 #include "dtypes.h"
 
@@ -323,14 +323,16 @@ __global__ __launch_bounds__(256) void token_group_kernel(const SumArgs a) {
 // n <= SMALL_MAX: a workgroup owns `rows` consecutive rows of the table and 64 * N columns.  It looks at all tokens and lists
 // the positions of its rows, in order; a wave sums and writes one row at a time, and rows of more than SMALL_ALONE positions
 // are left for all sixteen waves: each sums its sixteenth of the list, and the sums are added in order.  One launch instead of
-// a sort, groups and rows: at these sizes a launch costs the host (4 us) as much as the work takes.  Measured with events (some
-// 5 us of them the events'), words of falling frequency, against the three launches: 1280 words, 5000 x 512 fp32, 16.8 and 20.7
-// us; 2049 words, 432 x 301 fp16, 16.6 and 26.0; 4096 words, 5000 x 512 fp32, 31.5 and 28.6, and 8 us less of the host.  Above
-// SMALL_TABLE the workgroups no longer run side by side, and the looking at all tokens shows: 256 words, 50000 x 1024 bf16,
-// 48.3 and 27.4 us.
+// a sort, groups and rows: at these sizes a launch costs the host (4 us) as much as the work takes.  Every workgroup looks at all
+// tokens, so it is for tables of at most SMALL_GROUPS workgroups of SMALL_ROWS rows and 256 columns, or a narrower table's width:
+// two for every CU, which run side by side.  Measured with events (some 5 us of them the events'), words of falling frequency,
+// this launch and the sort's several: 5000 x 512 fp32, 5 words 11.1 and 11.8 us, 256 12.0 and 16.0, 1280 17.0 and 20.6, 4096 28.0 and
+// 26.8, and 8 us less of the host; 432 x 301 fp16, 2049 words, 16.6 and 26.0.  At the limit: 32768 x 64 fp32, 5 words 12.8 and 11.6,
+// 1280 17.8 and 21.6, 4096 27.4 and 24.8.  Above it the other way round: 65536 x 32 fp32 (1024 workgroups) 20.0 and 11.7, 24.2 and
+// 21.3, 37.9 and 25.0; 2^20 x 8 (16384) 217 and 33, 225 and 43, 241 and 47; 50000 x 1024 bf16, 256 words, 48.3 and 27.4.
 constexpr int SMALL_MAX = 4096;
 constexpr int SMALL_ROWS = 64;
-constexpr int64_t SMALL_TABLE = 1 << 23;   // elements: two workgroups of SMALL_ROWS rows and 256 columns for every CU
+constexpr int64_t SMALL_GROUPS = 512;
 constexpr int SMALL_WAVES = 16;
 constexpr int SMALL_ALONE = 128;            // positions that a wave adds up by itself: eight times 16 on their way
 
@@ -584,7 +586,7 @@ struct BwdSpace {
 
 BwdSpace bwd_space(int64_t n, int64_t vocab, int width) {
   BwdSpace s = {};
-  s.small = n <= SMALL_MAX && vocab * width <= SMALL_TABLE;
+  s.small = n <= SMALL_MAX && (vocab + SMALL_ROWS - 1) / SMALL_ROWS * ((width + 255) / 256) <= SMALL_GROUPS;
   if (s.small) return s;                                // (no workspace)
   s.rank = n <= RANK_MAX;
   int bits = 1;

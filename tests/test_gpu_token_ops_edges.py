@@ -49,3 +49,21 @@ def test_beam_select_orders_beams_that_are_close(V, dtype):
         assert torch.equal((parent - first)[apart], beam[apart]) and torch.equal(got[apart], word[apart])
         places = (parent * V + got).sort(dim=1)[0]
         assert bool((places[:, 1:] > places[:, :-1]).all())                       # no candidate twice
+
+
+# -------------------------------------------------------------------------------------------------------------- embedding
+@pytest.mark.parametrize('n', [1, 5, 300, 4096])
+@pytest.mark.parametrize('V,E', [(32768, 32), (32769, 32), (131072, 33), (1 << 20, 8), (1 << 21, 1), (200, 70001), (65, 1 << 17)])
+def test_embedding_gradient_of_narrow_and_wide_tables(V, E, n):
+    """Few tokens of tables on both sides of the rule that chooses the one-launch gradient.  The numbers are small multiples of a
+    power of two, so that sums in any order are exact."""
+    g = gen(n + V)
+    tok = torch.randint(0, V, (n,), generator=g, device='cuda') * (torch.rand(n, generator=g, device='cuda') < 0.5)
+    w = torch.randint(-4, 5, (V, E), generator=g, device='cuda').float().requires_grad_()
+    dy = torch.randint(-8, 9, (n, E), generator=g, device='cuda').float()
+    grad, = torch.autograd.grad(ops.embedding(tok, w, scale=0.5, act=1), w, dy)
+    used = torch.unique(tok)
+    want = torch.zeros(len(used), E, device='cuda').index_add_(0, torch.searchsorted(used, tok), dy) * 0.5 * (w.detach()[used] > 0)
+    assert torch.equal(grad[used], want)
+    grad[used] = 0
+    assert not bool(grad.any())

@@ -44,3 +44,14 @@ def test_embedding_workspace_is_what_the_function_says():
         for ws, size in ((None, need), (a, need - 1), (None, 0)):
             assert l.gvd_embedding_bwd(a, 1, n, a, width, a, width, vocab, width, 0, 1.0, 0, -1, a, ws, size, None) == -1
     assert l.gvd_embedding_bwd_workspace_bytes(4096, 5000, 512) == 0 == l.gvd_embedding_bwd_workspace_bytes(1, 1, 1)
+
+
+def test_embedding_one_launch_is_for_tables_of_few_workgroups():
+    """Every workgroup of the one-launch gradient looks at all tokens, so it is for tables of at most 512 of them (64 rows x 256
+    columns, or a narrower table's whole width): narrow tables of many rows are sorted for."""
+    need = hip.lib().gvd_embedding_bwd_workspace_bytes
+    for n in (5, 4096):
+        for vocab, width in ((32768, 32), (32768, 256), (32768, 1), (16384, 512), (8192, 1024), (5000, 512), (64, 1 << 17)):
+            assert need(n, vocab, width) == 0, (n, vocab, width)
+        for vocab, width in ((32769, 32), (131072, 32), (1 << 20, 8), (1 << 23, 1), (27000, 300), (32768, 257), (65, 1 << 17)):
+            assert need(n, vocab, width) > 0, (n, vocab, width)
