@@ -1,12 +1,14 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens.
 //
 //   forward    out[n,:] = act(scale * W[tok[n],:])
-//   backward   dW[v,:]  = scale * act'(scale * W[v,:]) * sum over n with tok[n] = v, n ascending, of dy[n,:]
+//   backward   dW[v,:]  = scale * act'(scale * W[v,:]) * sum over n with tok[n] = v of dy[n,:]
 //
 // (act' depends on the table row alone, so it multiplies the finished sum once.)  Both directions are bound by the rows they
 // move: out / dy once, the table's rows once.  The backward never adds with atomics: the positions are sorted by token (stable;
-// few, of a small table, are listed by token instead), every row of dW is summed by one owner in a fixed order and written once, rows
-// without a token as zeros.  Sums are fp32.
+// few, of a small table, are listed by token instead), every row of dW is summed by one owner in a fixed order and written once,
+// rows without a token as zeros.  The order is that of the positions, but for frequent words, whose groups of positions are
+// summed first (64 positions or more; in the form for few tokens more than 128): it depends on n and the table's size, not
+// on the run.  Sums are fp32.
 #include "dtypes.h"
 
 namespace {
@@ -243,8 +245,9 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
 
 // ------------------------------------------------------------------------------------------------------- sums by token
 // A token of 64 positions or more has its whole groups of GROUP sorted positions (and of GROUP groups) summed beforehand, one
-// wave per group with 16 rows on their way, so that no owner of a row adds up more than a few hundred rows whatever the tokens
-// are (131072 positions of 2048 bf16, half of them in such tokens: 50 us, 5.2 TB/s).
+// wave per group with 16 rows on their way, so that the owner of a row adds up m / 1024 + some 124 rows of a token of m positions
+// - a few hundred for the largest batches of texts; all of 2^25 tokens the same: 32768 + 124 (131072 positions of 2048 bf16, half of
+// them in such tokens: 50 us, 5.2 TB/s).
 constexpr int GROUP = 32;
 constexpr int STRETCH = 32;               // 8, 16 and 32 take the same time, 64 up to a fifth more
 

@@ -4,7 +4,7 @@
 //   dst  = factor * g     (in place, or into other tensors: 16-bit gradients of a scaled loss into fp32 master gradients)
 //
 // Bound by memory: the norm has to be known before the first element is written, so the gradients are read twice and written
-// once.  Squares and sums are fp64 - gradients from 1e-150 to 1e150 neither vanish nor overflow in the norm - and added in a
+// once.  Squares and sums are fp64 - no gradient that fp32 holds, 1e-45 to 3e38, vanishes or overflows in them - and added in a
 // fixed order (no atomics).  Two kinds of launch: gvd_grad_sumsq leaves one partial sum per workgroup; in gvd_grad_scale every
 // workgroup adds up all the partials by itself, in the same order, so no launch is spent on joining them.
 //
