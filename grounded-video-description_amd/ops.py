@@ -2080,6 +2080,8 @@ def reorder_rows(states, parent, dim=0, out=None):
         if not -x.dim() <= dim < x.dim():
             raise GvdHipError('reorder_rows: state %d has %d dimensions, no dimension %d' % (i, x.dim(), dim))
         d = dim % x.dim()
+        if x.is_conj() or x.is_neg():                # (lazy: the memory holds other values)
+            x = x.resolve_conj().resolve_neg()
         if rows is None:
             rows = x.shape[d]
         if x.shape[d] != rows:
@@ -2091,6 +2093,8 @@ def reorder_rows(states, parent, dim=0, out=None):
             y = out[i]
             if y.shape != shape or y.dtype != x.dtype or y.device != dev:
                 raise GvdHipError('reorder_rows: result %d must be %s %s on %s' % (i, x.dtype, tuple(shape), dev))
+            if y.is_conj() or y.is_neg():
+                raise GvdHipError('reorder_rows: result %d is a conjugated or negated view' % i)
         results.append(y)
         if y.numel() == 0:
             continue

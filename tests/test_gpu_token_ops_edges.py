@@ -1,8 +1,9 @@
-"""-m gpu: edges of the token-side operators - beams that lie closer together than fp32 tells apart."""
+"""-m gpu: edges of the token-side operators - beams that lie closer together than fp32 tells apart, narrow and wide tables, states
+whose memory holds other values than they stand for."""
 import pytest
 import torch
 
-from gvd_amd import ops
+from gvd_amd import hip, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,21 @@ def test_embedding_gradient_of_narrow_and_wide_tables(V, E, n):
     assert torch.equal(grad[used], want)
     grad[used] = 0
     assert not bool(grad.any())
+
+
+# ----------------------------------------------------------------------------------------------------------- reorder_rows
+def test_reorder_of_conjugated_and_negated_views():
+    """Views whose values are not what their memory holds (lazy conjugation and negation) come out as index_select's."""
+    p = torch.tensor([3, 0, 0, 2], device='cuda')
+    z = torch.randn(2, 4, 5, generator=gen(1), device='cuda', dtype=torch.complex64)
+    for x, d in ((z.conj(), 1), (z[0].conj(), 0), (z.conj().imag[:, :, 2], 1), (torch._neg_view(z.real.contiguous()), 1)):
+        assert x.is_conj() or x.is_neg()
+        got, = ops.reorder_rows([x], p, dim=d)
+        want = x.index_select(d, p)
+        assert torch.equal(got, want)
+        out = torch.empty_like(want)
+        ops.reorder_rows([x], p, dim=d, out=[out])
+        assert torch.equal(out, want)
+    for out in (torch.empty_like(z).conj(), torch._neg_view(torch.empty(2, 4, 5, device='cuda'))):
+        with pytest.raises(hip.GvdHipError, match='conjugated or negated'):
+            ops.reorder_rows([z if out.is_complex() else z.real], p, dim=1, out=[out])
