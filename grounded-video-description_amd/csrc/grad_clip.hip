@@ -86,8 +86,16 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(const gvd_grad_group g,
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// the factor as a product of two: one that fp32 holds as a normal number, and a power of two (1 but for norms over 2^100)
-struct Factor { float f, p; };
+// the factor as f 2^e: f is a normal fp32 number (or 0), e is 0 but for factors under 2^-100 (large norms) and over 2^100 (tiny loss
+// scales, where f is at least 2^63 and so no product of it is subnormal)
+struct Factor { float f; int e; };
+__device__ __forceinline__ Factor factor_of(double factor) {
+  int e = 0;
+  if (factor < 0x1p-100) factor = frexp(factor, &e);
+  else if (factor > 0x1p100) { factor = frexp(factor, &e) * 0x1p64; e -= 64; }
+  return {(float)factor, e};
+}
+__device__ __forceinline__ float operator*(float x, Factor f) { return ldexpf(x * f.f, f.e); }
 
 template <bool PAST, typename TI, typename TO>
 __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, Factor f) {
@@ -103,7 +111,7 @@ __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, F
     for (int i = 0; i < VECS; ++i) {
       float v[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = (float)x[i][k] * f.f * f.p;
+      for (int k = 0; k < N; ++k) v[k] = (float)x[i][k] * f;
       if constexpr (PAST) gvd_store_past<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
       else gvd_store<TO, N>(dst + (i * 256 + threadIdx.x) * N, v);
     }
@@ -114,10 +122,10 @@ __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, F
     float v[N];
     gvd_load<TI, N>(src + i, v);
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = v[k] * f.f * f.p;
+    for (int k = 0; k < N; ++k) v[k] = v[k] * f;
     gvd_store<TO, N>(dst + i, v);
   }
-  for (int64_t i = nv + threadIdx.x; i < n; i += 256) dst[i] = (TO)((float)src[i] * f.f * f.p);
+  for (int64_t i = nv + threadIdx.x; i < n; i += 256) dst[i] = (TO)((float)src[i] * f);
 }
 
 // Chunk k of a tensor.  Its chunks begin where the destination begins a 128-byte line (the first one holds what lies before,
@@ -125,7 +133,7 @@ __device__ __forceinline__ void chunk_scale(const TI* src, TO* dst, int64_t n, F
 template <bool PAST, typename TI, typename TO>
 __device__ __forceinline__ void scale_chunk(const TI* src, TO* dst, int64_t k, int64_t n, Factor f) {
   const int64_t before = (int64_t)((128u - (unsigned)(reinterpret_cast<uintptr_t>(dst) & 127u)) % 128u / sizeof(TO));
-  if (k == 0 && threadIdx.x < before && threadIdx.x < n) dst[threadIdx.x] = (TO)((float)src[threadIdx.x] * f.f * f.p);
+  if (k == 0 && threadIdx.x < before && threadIdx.x < n) dst[threadIdx.x] = (TO)((float)src[threadIdx.x] * f);
   const int64_t e0 = k * CHUNK + before, e1 = e0 + CHUNK < n ? e0 + CHUNK : n;
   if (e0 < e1) chunk_scale<PAST>(src + e0, dst + e0, e1 - e0, f);
 }
@@ -147,8 +155,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const gvd_grad_group g,
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const double clip = c.max_norm / (norm + 1e-6);
   const double factor = (clip > 1.0 ? 1.0 : clip) * c.inv_scale;           // (a NaN norm makes every gradient NaN)
-  const bool tiny = factor < 0x1p-100;
-  const Factor f = {(float)(tiny ? factor * 0x1p100 : factor), tiny ? 0x1p-100f : 1.0f};
+  const Factor f = factor_of(factor);
   const unsigned chunks = g.count ? g.chunk0[g.count] : 0;
   const FirstChunks first(g);
   // from the last chunk to the first: what gvd_grad_sumsq read last is still in the 256 MB cache

@@ -1,9 +1,9 @@
 """-m gpu: edges of the token-side operators - beams that lie closer together than fp32 tells apart, narrow and wide tables, states
-whose memory holds other values than they stand for."""
+whose memory holds other values than they stand for, loss scales past fp32's range."""
 import pytest
 import torch
 
-from gvd_amd import hip, ops
+from gvd_amd import hip, ops, optim
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,19 @@ def test_reorder_of_conjugated_and_negated_views():
     for out in (torch.empty_like(z).conj(), torch._neg_view(torch.empty(2, 4, 5, device='cuda'))):
         with pytest.raises(hip.GvdHipError, match='conjugated or negated'):
             ops.reorder_rows([z if out.is_complex() else z.real], p, dim=1, out=[out])
+
+
+# ------------------------------------------------------------------------------------------------------------------- clip
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+@pytest.mark.parametrize('inv', [1e30, 1e39, 1e100])
+def test_clip_by_factors_over_the_range_of_fp32(inv, dtype):
+    """A loss scale far under 1: the factor does not fit fp32, products that do come out, zeros stay zeros, the rest is infinite."""
+    g = torch.tensor([0.0, -0.0, 2.0 ** -24, -2.0 ** -14, 1.0], device='cuda').to(dtype)
+    out = torch.full((5,), 7.0, device='cuda')
+    norm = optim.clip_grads([g], float('inf'), out=[out], inv_scale=inv)
+    want = g.double() * inv
+    big = want.abs() > torch.finfo(torch.float32).max
+    assert torch.equal(torch.isinf(out), big) and torch.equal(torch.signbit(out), torch.signbit(want))
+    # the factor, the product and a power of two: two roundings (values here are no subnormal numbers)
+    assert bool(((out.double() - want).abs()[~big] <= want.abs()[~big] * 2.01 * 2.0 ** -24).all())
+    assert float(norm) == float((g.double().square().sum().sqrt() * inv).float())
