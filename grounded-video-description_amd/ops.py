@@ -1944,7 +1944,7 @@ def embedding(tokens, weight, scale=1.0, act=0, padding_idx=None):
     act 1 = ReLU; padding_idx: a row that gets no gradient.  The result has weight's type, [..., E], rounded once.
     Gradient: positions sorted by token, every row of the table summed in fp32 in a fixed order - the same bits at every
     run - and written once.  A token outside [0, V) is not an error the host can see without waiting: its row of the result
-    is NaN and it adds nothing to the gradient.  At most 2^25 tokens and rows."""
+    is NaN and it adds nothing to the gradient.  At most 2^25 tokens and rows, 2^20 columns, a result of less than 256 GiB."""
     pad = _check_embedding(tokens, weight, act, padding_idx)
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     V, E = weight.shape
@@ -1967,7 +1967,7 @@ def beam_select(logits, scores, width=None, finished=None, eos=None):
 
     Returns (scores f32 [B, W], parent i64 [B, W], word i64 [B, W], finished [B, W]): parent = the row b*K + q the candidate
     extends, as reorder_rows takes it; finished = of the type given (u8 if none was), None without eos.
-    K, W <= 32; B * K <= 65535.  Not differentiable."""
+    K, W <= 32; B * K <= 65535; V <= 2^28.  Not differentiable."""
     if logits.dtype not in DTYPES or scores.dtype != torch.float32 or scores.dim() != 2:
         raise GvdHipError('beam_select: logits must be float32 / bfloat16 / float16 and scores float32 [B, K], got %s and %s %s'
                           % (logits.dtype, scores.dtype, tuple(scores.shape)))
@@ -2058,8 +2058,9 @@ def reorder_rows(states, parent, dim=0, out=None):
     states: tensors of any type whose dimension `dim` holds the same number of rows; parent int64, any shape (its entries in
     order are the new rows: beam_select's parent goes in as it is).  out: tensors of the result's shape and type, which must not
     overlap the states or parent (two sets of buffers, swapped from step to step); otherwise new ones.  Returns the list of results.
-    A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1).  Not
-    differentiable: the results carry no gradient."""
+    A parent outside the rows is not an error the host can see without waiting: its rows get all bits set (NaN, -1).  At
+    most 128 GiB of results for 16 states; states of rows under 16 KiB: 32 GiB each (rows of 16 bytes or more; shorter ones 2^31
+    numbers of 8, 4 or 1 bytes).  Not differentiable: the results carry no gradient."""
     states = list(states)
     dev = parent.device
     if parent.dtype != torch.int64:

@@ -713,7 +713,7 @@ int gvd_adam_step(const gvd_opt_group* g, const float* clip, const int* skip, in
 /* Embedding lookup: out[i,:] = act(scale * table[tokens[i],:]), i < n.  tokens: int64 (tok64 != 0) or int32, contiguous;
  * table [vocab, width] (row stride ld), out [n, width] (row stride ldo), both of type dtype, elements of a row contiguous; act: 0
  * none, 1 ReLU.  A token outside [0, vocab) reads nothing; its row of out is NaN.
- * Limits: n, vocab <= GVD_EMBEDDING_MAX, width <= 2^20. */
+ * Limits: n, vocab <= GVD_EMBEDDING_MAX, width <= 2^20, an out of less than 256 GiB. */
 #define GVD_EMBEDDING_MAX (1 << 25)
 int gvd_embedding_fwd(const void* tokens, int tok64, int64_t n, const void* table, int64_t ld, int64_t vocab, int width, int dtype,
                       float scale, int act, void* out, int64_t ldo, gvd_stream_t stream);
@@ -759,7 +759,8 @@ int gvd_grad_scale(const gvd_grad_group* g, const gvd_grad_clip* c, const void* 
  *   cand[q,v] = scores[b,q] + (logits[b*K+q, v] - log sum_v exp(logits[b*K+q, v]))
  * in descending order, equal ones by q * V + v ascending, computed and compared in fp64 (words of one beam: by their logits).
  * finished (nullable, u8 [B,K]): an ended beam has scores[b,q] for the word eos and -inf for the others; its logits do
- * not matter.  A beam whose score or log-sum-exp is not finite has -inf for every word.  logits [B*K, V] of type dtype, row stride ld.
+ * not matter.  A beam whose score or log-sum-exp is not finite has -inf for every word.  logits [B*K, V] of type dtype, row
+ * stride ld.
  * Out, [B,W] each: out_scores f32, parent = b*K + q, word, out_finished = finished[b,q] or word == eos (nullable; eos = -1: none).
  * Limits: K, W <= GVD_BEAM_SELECT_MAX, W <= K * V, B * K <= 65535, V <= 2^28.
  * workspace: gvd_beam_select_workspace_bytes(B, K, V, W) bytes, 16-byte aligned, contents free. */
@@ -778,7 +779,9 @@ int gvd_beam_select(const gvd_beam_select_args* args, gvd_stream_t stream);
 /* Reordering of the beams' states: dst[o, r, :] = src[o, index[r], :] for up to GVD_REORDER_MAX_TENSORS tensors in one launch.
  * A tensor is [outer, rows, row_bytes] with the byte strides src_outer / src_row and dst_outer / dst_row; index int64
  * [rows_out], shared by the tensors.  A dst must not overlap a src, the index or another dst.  An index outside [0, rows_in) reads
- * nothing: its rows get all bits set (NaN, -1).  `unit` and `tile0` are filled in by the call. */
+ * nothing: its rows get all bits set (NaN, -1).  `unit` and `tile0` are filled in by the call.
+ * Limits: 128 GiB of rows a call; tensors of rows under 16 KiB: fewer than 2^31 - 1 units (16 bytes; rows under 16 bytes: 8, 4
+ * or 1) each. */
 #define GVD_REORDER_MAX_TENSORS 16
 typedef struct {
   const void* src; void* dst;
